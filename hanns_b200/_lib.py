@@ -70,6 +70,24 @@ class Artifact(C.Structure):
     ]
 
 
+class EmbedBags(C.Structure):
+    """hanns_embed_bags_t."""
+    _fields_ = [("dtype", C.c_int32), ("out_dtype", C.c_int32), ("dim", C.c_int32),
+                ("mean", C.c_int32), ("rows", C.c_int64), ("ld", C.c_int64),
+                ("n_tokens", C.c_int64), ("n_bags", C.c_int64), ("scale", C.c_float),
+                ("reserved", C.c_int32), ("table", vp), ("tokens", vp), ("offsets", vp),
+                ("weights", vp), ("out", vp), ("out_ld", C.c_int64), ("inv_counts", vp),
+                ("workspace", vp), ("workspace_bytes", C.c_int64)]
+
+
+class TokenLogprobs(C.Structure):
+    """hanns_token_logprobs_t."""
+    _fields_ = [("dtype", C.c_int32), ("top", C.c_int32), ("n", C.c_int64), ("vocab", C.c_int64),
+                ("ld", C.c_int64), ("temperature", C.c_float), ("reserved", C.c_int32),
+                ("logits", vp), ("tokens", vp), ("logprobs", vp), ("entropy", vp),
+                ("top_tokens", vp), ("top_logprobs", vp), ("stats", vp)]
+
+
 # Every symbol declared in include/hanns_gpu.h: (name, restype, argtypes)
 SIGNATURES = [
     ("knowhere_create_index", vp, [CIndexConfig]),
@@ -158,6 +176,16 @@ SIGNATURES = [
     ("hanns_gpu_ivf_usq_save_ivfusq00", C.c_int32, [vp, C.c_char_p, C.c_uint64, C.c_int64]),
     ("hanns_gpu_coarse_probes_static", C.c_int32,
      [vp, C.c_int64, vp, C.c_int32, C.c_int32, C.c_int32, vp, vp]),
+    ("hanns_gpu_embed_bags_workspace_bytes", C.c_int64, [C.POINTER(EmbedBags)]),
+    ("hanns_gpu_embed_bags_device", C.c_int32, [C.POINTER(EmbedBags), vp]),
+    ("hanns_gpu_embed_bags_grad_workspace_bytes", C.c_int64, [C.POINTER(EmbedBags)]),
+    ("hanns_gpu_embed_bags_grad_device", C.c_int32,
+     [C.POINTER(EmbedBags), vp, C.c_int64, vp, C.c_int64, vp, vp]),
+    ("hanns_gpu_token_logprobs_device", C.c_int32, [C.POINTER(TokenLogprobs), vp]),
+    ("hanns_gpu_token_logprobs_grad_device", C.c_int32,
+     [C.POINTER(TokenLogprobs), vp, vp, vp, vp, C.c_int64, vp]),
+    ("hanns_gpu_neighbour_logprobs_device", C.c_int32,
+     [C.POINTER(TokenLogprobs), vp, vp, C.c_int32, vp, C.c_int64, C.c_float, C.c_float, vp]),
 ]
 
 _lib = None

@@ -23,9 +23,10 @@ LIB = os.path.join(OUT_DIR, "libhanns_gpu.so")
 OBJ_DIR = os.path.join(HERE, "_build")
 
 CU_SOURCES = ["search_kernels.cu", "build_kernels.cu", "ivf_usq_gpu.cu", "capi.cu",
-              "coarse_static.cu", "coarse_tc.cu", "scan_tc.cu"]
+              "coarse_static.cu", "coarse_tc.cu", "scan_tc.cu", "embed_bags.cu",
+              "token_logprobs.cu"]
 CPP_SOURCES = ["rotation.cpp", "ivfusq00.cpp"]
-HEADERS = ["common.cuh", "kernels.h", "ivf_usq_gpu.h", "warp_select.cuh"]
+HEADERS = ["common.cuh", "kernels.h", "ivf_usq_gpu.h", "warp_select.cuh", "operators.cuh"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

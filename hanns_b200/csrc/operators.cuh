@@ -1,0 +1,71 @@
+// operators.cuh -- what the language-model operators (embed_bags.cu, token_logprobs.cu) share:
+// element types, vector loads that convert to f32, and the guard of their C entry points.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <stdexcept>
+#include <string>
+
+#include "common.cuh"
+#include "hanns_gpu.h"
+#include "ivf_usq_gpu.h"
+
+namespace hanns {
+
+void set_last_error(const std::string& msg);
+
+// Runs f and maps what it throws to the CError codes of the C ABI.
+template <class F>
+int32_t operator_entry(F&& f) {
+    try {
+        f();
+        return HANNS_OK;
+    } catch (const std::invalid_argument& e) {
+        set_last_error(e.what());
+        return HANNS_INVALID_ARG;
+    } catch (const CudaError& e) {
+        set_last_error(e.what());
+        return e.code == cudaErrorMemoryAllocation ? HANNS_OUT_OF_MEMORY : HANNS_INTERNAL;
+    } catch (const std::exception& e) {
+        set_last_error(e.what());
+        return HANNS_INTERNAL;
+    } catch (...) {
+        set_last_error("unknown error");
+        return HANNS_INTERNAL;
+    }
+}
+
+inline void require(bool ok, const char* what) {
+    if (!ok) throw std::invalid_argument(what);
+}
+
+inline int dtype_bytes(int32_t dtype) { return dtype == HANNS_DTYPE_F32 ? 4 : 2; }
+inline bool dtype_known(int32_t dtype) {
+    return dtype == HANNS_DTYPE_F32 || dtype == HANNS_DTYPE_F16 || dtype == HANNS_DTYPE_BF16;
+}
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+// One rounding to nearest even, the only one between the f32 sums and a 16-bit result.
+template <class T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+    return __float2bfloat16_rn(v);
+}
+
+// N elements of T moved by one access (N * sizeof(T) is 16, 8, 4 or 2 bytes).
+template <class T, int N>
+struct alignas(sizeof(T) * N) Pack {
+    T v[N];
+};
+
+template <class T, int N>
+__device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
+    return *reinterpret_cast<const Pack<T, N>*>(p);
+}
+
+}  // namespace hanns

@@ -249,6 +249,70 @@ class IvfUsqIndex:
             n_bitsets, d_query_bitset or None, d_ids, d_dists, d_counts or None, stream or None),
             "search_device")
 
+    def _search_tensors(self, queries, k: int, nprobe: int):
+        """Rows (ids, distances) of f32 device queries as device tensors, in the order of the
+        current stream.  The library runs calls on the legacy default stream synchronously,
+        so a call made there goes through a stream of the index's own."""
+        import torch
+        dev = torch.device("cuda", self.device)
+        ids = torch.empty(queries.shape[0], k, dtype=torch.int64, device=dev)
+        dists = torch.empty(queries.shape[0], k, dtype=torch.float32, device=dev)
+        if queries.shape[0] == 0:
+            return ids, dists
+        cur = torch.cuda.current_stream(dev)
+        run = cur
+        if cur.cuda_stream == 0:
+            if getattr(self, "_tensor_stream", None) is None:
+                self._tensor_stream = torch.cuda.Stream(dev)
+            run = self._tensor_stream
+            run.wait_stream(cur)
+        self.search_device(queries.data_ptr(), queries.shape[0], k, nprobe, ids.data_ptr(),
+                           dists.data_ptr(), stream=run.cuda_stream)
+        if run is not cur:
+            cur.wait_stream(run)
+        return ids, dists
+
+    def _check_vectors(self, t, what: str):
+        if not t.is_cuda or t.device.index != self.device:
+            raise ValueError(f"{what} must be on cuda:{self.device}, not {t.device}")
+        if t.shape[-1] != self.config.dim:
+            raise ValueError("query dimension mismatch")
+
+    def search_tokens(self, table, tokens, offsets, req: SearchRequest, weights=None, *,
+                      scale: float = 1.0, mean: bool = True):
+        """Searches for bags of token ids: embeds them (hanns_b200.embed_bags, f32 vectors from
+        `table`) and searches the vectors, all on the device.  Returns the torch tensors (ids,
+        distances), [bags, top_k] each, in the order of the current stream."""
+        from .tokens import embed_bags
+        import torch
+        if offsets is None:
+            raise ValueError("search_tokens needs offsets")
+        self._check_vectors(table, "table")
+        with torch.no_grad():
+            q = embed_bags(table, tokens, offsets, weights, scale=scale, mean=mean,
+                           out_dtype=torch.float32)
+            return self._search_tensors(q, max(int(req.top_k), 1), max(int(req.nprobe), 1))
+
+    def token_logprobs(self, queries, logits, tokens, values, req: SearchRequest, *,
+                       weight: float = 0.25, knn_temperature: float = 1.0, top: int = 0,
+                       temperature: float = 1.0):
+        """Nearest-neighbour language modelling: searches the index for each row's context vector
+        (queries, [..., dim] f32 on the device) and scores `tokens` under the mixture of the
+        model's logits with the tokens that `values` gives the found ids
+        (hanns_b200.token_logprobs with Neighbours).  Scoring only."""
+        from .tokens import Neighbours, token_logprobs
+        import torch
+        self._check_vectors(queries, "queries")
+        if queries.dtype != torch.float32 or queries.shape[:-1] != tokens.shape:
+            raise ValueError("queries must be float32, one vector per token")
+        k = max(int(req.top_k), 1)
+        with torch.no_grad():
+            flat = queries.reshape(-1, self.config.dim).contiguous()
+            ids, dists = self._search_tensors(flat, k, max(int(req.nprobe), 1))
+            near = Neighbours(ids.reshape(*tokens.shape, k), dists.reshape(*tokens.shape, k), values,
+                              weight, knn_temperature)
+            return token_logprobs(logits, tokens, top=top, temperature=temperature, neighbours=near)
+
     def rerank_rows(self, queries: np.ndarray, rows: np.ndarray) -> np.ndarray:
         """USQ distances of stored rows (storage order, as export_artifact lists them):
         rows[q, j] for query q; rows outside [0, count) give +inf.  The score_with_meta

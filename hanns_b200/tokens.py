@@ -1,0 +1,309 @@
+"""Language-model operators beside the search, on torch CUDA tensors.
+
+embed_bags      token ids -> vectors to search with (or to add), from an embedding table
+token_logprobs  log probabilities of given tokens from logits, their entropy and the most likely
+                alternatives; with `neighbours` those of the mixture with what a search found
+
+Both go through the C ABI (hanns_gpu_embed_bags_*, hanns_gpu_token_logprobs_*,
+hanns_gpu_neighbour_logprobs_device), run on the current stream of the tensors' device,
+take their scratch from torch's allocator and are differentiable once.  Bad arguments raise
+ValueError, GPU failures RuntimeError.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass
+from typing import NamedTuple
+
+import torch
+
+from . import _lib as L
+
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _check(rc: int, what: str):
+    if rc != 0:
+        msg = L.last_error()
+        if rc == 2:
+            raise ValueError(f"{what}: {msg}")
+        raise RuntimeError(f"{what} failed ({rc}): {msg}")
+
+
+def _need(ok, what: str):
+    if not ok:
+        raise ValueError(what)
+
+
+def _on(t, device, name):
+    _need(isinstance(t, torch.Tensor), f"{name} must be a tensor")
+    _need(t.device == device, f"{name} must be on {device}, not {t.device}")
+
+
+def _cuda(t, name):
+    _need(isinstance(t, torch.Tensor), f"{name} must be a tensor")
+    _need(t.dtype in _DTYPES, f"{name} must be float32, float16 or bfloat16, not {t.dtype}")
+    _need(t.is_cuda, f"{name} must be on a CUDA device, not {t.device}")
+
+
+def _ids(t, device, name):
+    _on(t, device, name)
+    _need(t.dtype in (torch.int64, torch.int32), f"{name} must be int64 or int32, not {t.dtype}")
+    return t.to(torch.int64).contiguous()
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _rows(t):
+    """t with its last dimension dense, or a copy (rows may be any distance apart)."""
+    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _workspace(nbytes, device):
+    if nbytes < 0:
+        raise ValueError(f"embed_bags: {L.last_error()}")
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+# ---------------------------------------------------------------------------- embed_bags
+def _bags(table, tokens, offsets, weights, scale, mean, out_dtype, inv_counts):
+    b = L.EmbedBags()
+    b.dtype, b.out_dtype = _DTYPES[table.dtype], _DTYPES[out_dtype]
+    b.rows, b.dim = table.shape
+    b.ld, b.mean, b.scale = table.stride(0), int(mean), scale
+    b.n_tokens = tokens.numel()
+    b.n_bags = b.n_tokens if offsets is None else offsets.numel() - 1
+    b.table, b.tokens, b.offsets = _ptr(table), _ptr(tokens), _ptr(offsets)
+    b.weights, b.inv_counts = _ptr(weights), _ptr(inv_counts)
+    return b
+
+
+def _embed_bags(table, tokens, offsets, weights, scale, mean, out_dtype, keep):
+    """The vectors, and with `keep` what a mean's gradient needs (1 / c_i)."""
+    dev = table.device
+    n_bags = tokens.numel() if offsets is None else offsets.numel() - 1
+    inv = torch.empty(n_bags, dtype=torch.float32, device=dev) if mean and keep else None
+    out = torch.empty(n_bags, table.shape[1], dtype=out_dtype, device=dev)
+    b = _bags(table, tokens, offsets, weights, scale, mean, out_dtype, inv)
+    b.out, b.out_ld = _ptr(out), out.stride(0)
+    with torch.cuda.device(dev):
+        ws = _workspace(L.lib().hanns_gpu_embed_bags_workspace_bytes(C.byref(b)), dev)
+        b.workspace, b.workspace_bytes = _ptr(ws), 0 if ws is None else ws.numel()
+        _check(L.lib().hanns_gpu_embed_bags_device(C.byref(b), _stream(dev)), "embed_bags")
+    return out, inv
+
+
+class _EmbedBags(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, tokens, offsets, weights, scale, mean, out_dtype):
+        out, inv = _embed_bags(table, tokens, offsets, weights, scale, mean, out_dtype, True)
+        ctx.save_for_backward(table, tokens, offsets, weights, inv)
+        ctx.args = scale, mean, out_dtype
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        d_table, d_weights = _embed_bags_grad(grad, *ctx.saved_tensors, *ctx.args,
+                                              ctx.needs_input_grad[0], ctx.needs_input_grad[3])
+        return d_table, None, None, d_weights, None, None, None
+
+
+def _embed_bags_grad(grad, table, tokens, offsets, weights, inv, scale, mean, out_dtype, want_table,
+                     want_weights):
+    dev = table.device
+    grad = _rows(grad)
+    d_table = d_weights = None
+    if want_table:
+        d_table = torch.empty(table.shape, dtype=table.dtype, device=dev)
+    if want_weights:
+        d_weights = torch.empty(tokens.numel(), dtype=torch.float32, device=dev)
+    b = _bags(table, tokens, offsets, weights, scale, mean, out_dtype, inv)
+    with torch.cuda.device(dev):
+        ws = None
+        if want_table:
+            ws = _workspace(L.lib().hanns_gpu_embed_bags_grad_workspace_bytes(C.byref(b)), dev)
+        b.workspace, b.workspace_bytes = _ptr(ws), 0 if ws is None else ws.numel()
+        _check(L.lib().hanns_gpu_embed_bags_grad_device(
+            C.byref(b), _ptr(grad), grad.stride(0), _ptr(d_table),
+            d_table.stride(0) if want_table else 0, _ptr(d_weights), _stream(dev)), "embed_bags")
+    return d_table, d_weights
+
+
+def embed_bags(table, tokens, offsets=None, weights=None, *, scale: float = 1.0, mean: bool = False,
+               out_dtype=None):
+    """Bags of token ids to vectors:
+
+        out[i] = scale / c_i * sum over bag i's tokens t_j of weights[j] * table[t_j]
+
+    table      [rows, dim], float32, float16 or bfloat16; rows may be strided
+    tokens     int64 or int32 ids.  With `offsets` one-dimensional: bag i is
+               tokens[offsets[i]:offsets[i + 1]].  Without, any shape: every token is a bag
+               (a lookup), and the result has the shape tokens.shape + (dim,)
+    offsets    ascending int64 or int32 [bags + 1], or None
+    weights    float32 [len(tokens)] factors, or None
+    mean       divide by c_i, the bag's counted tokens (else c_i = 1)
+    out_dtype  the table's type (default) or float32, which IvfUsqIndex searches
+
+    A token outside [0, rows) is not counted (-1 pads, as in search results); an empty bag
+    gives zeros; positions outside every bag are not read.  Sums are f32, rounded once.
+    Differentiable in table (a dense gradient) and weights; the gradients add a token's terms in
+    the order of its positions and do not change from run to run.
+    """
+    _cuda(table, "table")
+    _need(table.dim() == 2 and table.shape[0] > 0 and table.shape[1] > 0, "table must be [rows, dim]")
+    dev = table.device
+    out_dtype = out_dtype or table.dtype
+    _need(out_dtype in (table.dtype, torch.float32), "out_dtype must be the table's type or float32")
+    tokens = _ids(tokens, dev, "tokens")
+    shape = tokens.shape
+    if offsets is None:
+        tokens = tokens.reshape(-1)
+    else:
+        _need(tokens.dim() == 1, "tokens must be one-dimensional when offsets are given")
+        offsets = _ids(offsets, dev, "offsets")
+        _need(offsets.dim() == 1 and offsets.numel() > 0, "offsets must be [bags + 1]")
+    if weights is not None:
+        _on(weights, dev, "weights")
+        _need(weights.dtype == torch.float32, "weights must be float32")
+        _need(weights.numel() == tokens.numel(), "weights must have one value per token")
+        weights = weights.reshape(-1).contiguous()
+    scale = float(scale)
+    _need(scale == scale and abs(scale) != float("inf"), "scale must be finite")
+    args = _rows(table), tokens, offsets, weights, scale, bool(mean), out_dtype
+    if torch.is_grad_enabled() and (table.requires_grad or weights is not None and weights.requires_grad):
+        out = _EmbedBags.apply(*args)
+    else:
+        out, _ = _embed_bags(*args, False)
+    return out.reshape(*shape, table.shape[1]) if offsets is None else out
+
+
+# ---------------------------------------------------------------------------- token_logprobs
+class TokenLogprobs(NamedTuple):
+    """logprobs and entropy have the tokens' shape, the alternatives one more dimension."""
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_tokens: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+@dataclass
+class Neighbours:
+    """What a search found for each row, and what it says about the next token.
+
+    ids, distances  [..., k] as the search returns them (smaller is nearer, -1 / +inf pads)
+    values          [stored ids] int64 or int32: the token that goes with each id
+    weight          share of the neighbours in the mixture, in [0, 1]
+    temperature     of softmax(-distance / temperature) over the neighbours
+    """
+    ids: torch.Tensor
+    distances: torch.Tensor
+    values: torch.Tensor
+    weight: float = 0.25
+    temperature: float = 1.0
+
+
+def _probs(logits, tokens, top, temperature, out):
+    t = L.TokenLogprobs()
+    t.dtype, t.top, t.temperature = _DTYPES[logits.dtype], top, temperature
+    t.n, t.vocab = logits.shape
+    t.ld = logits.stride(0)
+    t.logits, t.tokens = _ptr(logits), _ptr(tokens)
+    t.logprobs, t.entropy, t.top_tokens, t.top_logprobs, t.stats = (_ptr(o) for o in out)
+    return t
+
+
+def _token_logprobs(logits, tokens, top, temperature, near, keep):
+    """logprobs, entropy, top tokens, top logprobs and, with `keep`, the rows' statistics."""
+    dev, n = logits.device, logits.shape[0]
+    f32 = dict(dtype=torch.float32, device=dev)
+    out = (torch.empty(n, **f32), torch.empty(n, **f32),
+           torch.empty(n, top, dtype=torch.int64, device=dev), torch.empty(n, top, **f32),
+           torch.empty(n, 4, **f32) if keep or near is not None else None)
+    t = _probs(logits, tokens, top, temperature, out)
+    with torch.cuda.device(dev):
+        _check(L.lib().hanns_gpu_token_logprobs_device(C.byref(t), _stream(dev)), "token_logprobs")
+        if near is not None:
+            ids, distances, values, weight, knn_temperature = near
+            _check(L.lib().hanns_gpu_neighbour_logprobs_device(
+                C.byref(t), _ptr(ids), _ptr(distances), ids.shape[-1], _ptr(values), values.numel(),
+                weight, knn_temperature, _stream(dev)), "token_logprobs")
+    return out
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, top, temperature):
+        out = _token_logprobs(logits, tokens, top, temperature, None, True)
+        ctx.mark_non_differentiable(out[2])
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(logits, tokens, *out)
+        ctx.args = top, temperature
+        return out[:4]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logprobs, g_entropy, _, g_top):
+        logits, tokens, *out = ctx.saved_tensors
+        dev = logits.device
+        g = [None if x is None else x.to(torch.float32).contiguous() for x in (g_logprobs, g_entropy, g_top)]
+        d = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        t = _probs(logits, tokens, *ctx.args, out)
+        with torch.cuda.device(dev):
+            _check(L.lib().hanns_gpu_token_logprobs_grad_device(
+                C.byref(t), *(_ptr(x) for x in g), _ptr(d), d.stride(0), _stream(dev)), "token_logprobs")
+        return d, None, None, None
+
+
+def token_logprobs(logits, tokens, *, top: int = 0, temperature: float = 1.0,
+                   neighbours: Neighbours | None = None) -> TokenLogprobs:
+    """Log probabilities of given tokens under softmax(logits / temperature), the entropy of
+    that distribution, and its `top` most likely tokens.
+
+    logits  [..., vocab] float32, float16 or bfloat16; rows may be strided
+    tokens  [...] int64 or int32; a token outside [0, vocab) (-1 pads) gives 0 and no gradient
+    top     0 to 32 alternatives, larger logit first and ties to the lower token; (-1, -inf)
+            where fewer logits are unmasked
+
+    -inf masks a token.  A row of -inf alone gives log probability -inf, entropy 0 and no
+    alternatives (and a zero gradient); a row with NaN or +inf gives NaN.  Differentiable in
+    logits, through logprobs, entropy and top_logprobs.
+
+    With `neighbours` the distribution is (1 - weight) * model + weight * neighbours (nearest-
+    neighbour language modelling): a neighbour counts when its id is in [0, len(values)), its
+    distance is finite and its token is in the vocabulary and not masked; a row without such a
+    neighbour keeps the model's distribution.  Scoring only: not differentiable.
+    """
+    _cuda(logits, "logits")
+    _need(logits.dim() >= 1 and logits.shape[-1] > 0, "logits must be [..., vocab]")
+    dev, vocab = logits.device, logits.shape[-1]
+    tokens = _ids(tokens, dev, "tokens")
+    _need(tokens.shape == logits.shape[:-1], "tokens must have the shape of logits without its last dimension")
+    top, temperature = int(top), float(temperature)
+    _need(0 <= top <= 32, "top must be in [0, 32]")
+    near = None
+    if neighbours is not None:
+        _need(not (logits.requires_grad and torch.is_grad_enabled()),
+              "token_logprobs with neighbours is not differentiable: detach the logits")
+        ids = _ids(neighbours.ids, dev, "neighbours.ids")
+        _on(neighbours.distances, dev, "neighbours.distances")
+        _need(neighbours.distances.dtype == torch.float32, "neighbours.distances must be float32")
+        _need(ids.dim() >= 1 and ids.shape[:-1] == tokens.shape and ids.shape == neighbours.distances.shape,
+              "neighbours.ids and .distances must be tokens.shape + (k,)")
+        values = _ids(neighbours.values, dev, "neighbours.values")
+        _need(values.dim() == 1, "neighbours.values must be one-dimensional")
+        near = (ids, neighbours.distances.contiguous(), values, float(neighbours.weight),
+                float(neighbours.temperature))
+    args = _rows(logits).reshape(-1, vocab), tokens.reshape(-1), top, temperature
+    if torch.is_grad_enabled() and logits.requires_grad:
+        lp, h, tt, tl = _TokenLogprobs.apply(*args)
+    else:
+        lp, h, tt, tl, _ = _token_logprobs(*args, near, False)
+    s = tokens.shape
+    return TokenLogprobs(lp.reshape(s), h.reshape(s), tt.reshape(*s, top), tl.reshape(*s, top))

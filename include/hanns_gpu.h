@@ -1,7 +1,7 @@
 /*
  * hanns_gpu.h -- C ABI of libhanns_gpu.so, the B200 (sm_100a) IVF-USQ search library.
  *
- * Three groups of entry points:
+ * Four groups of entry points:
  *  1. The KnowHere C ABI of Hanns (reference src/ffi.rs), for the IVF-USQ index kind.
  *     Signatures, struct layouts, error codes and ownership rules are those of the
  *     reference; each declaration cites the reference item it replaces.
@@ -9,6 +9,8 @@
  *  3. hanns_gpu_* extras with no counterpart in the reference: artifact import and
  *     export (parity testing on a frozen index), device-pointer search, per-query
  *     bitsets, list sharding for multi-GPU and per-stage timings.
+ *  4. Language-model operators beside the search: token embedding bags and token log
+ *     probabilities, with their gradients.
  *
  * Every call returns NULL / an error code on failure and never aborts the process;
  * hanns_gpu_last_error() describes the last failure of the calling thread.
@@ -370,6 +372,91 @@ int32_t hanns_gpu_merge_shards_device(const float* d_dists, const uint64_t* d_ke
 int32_t hanns_gpu_coarse_probes_static(const float* d_queries, int64_t nq,
                                        const float* d_centroids, int32_t nlist, int32_t dim,
                                        int32_t nprobe, int32_t* d_probes, void* stream);
+
+/* ------------------------------------------------- language-model operators */
+/* The steps before and after the search where a language model is at hand; no counterpart in
+ * the reference.  Device pointers of the current device; stream-ordered on `stream`
+ * (cudaStream_t, NULL = the legacy default stream): a call returns once its work is enqueued,
+ * allocates nothing and may be captured into a graph.  Scratch is the caller's, sized by
+ * the matching *_workspace_bytes (-1 for bad arguments), 256-byte aligned; calls that may
+ * run at the same time need workspaces of their own. */
+#define HANNS_DTYPE_F32 0
+#define HANNS_DTYPE_F16 1
+#define HANNS_DTYPE_BF16 2
+
+/* Bags of tokens to vectors: out[i] = (scale / c_i) * sum over the tokens t_j of bag i of
+ * weights[j] * table[t_j], summed in f32, c_i = the bag's counted tokens for a mean, else 1.
+ * A token outside [0, rows) is not counted and adds nothing; an empty bag's row is zero.
+ * Bag i is tokens[offsets[i] .. offsets[i+1]), offsets ascending; positions outside every
+ * bag are not read.  offsets NULL: every token is its own bag (n_bags = n_tokens). */
+typedef struct {
+    int32_t dtype;     /* HANNS_DTYPE_* of the table */
+    int32_t out_dtype; /* the table's type, or f32 */
+    int32_t dim;
+    int32_t mean;      /* 0: sums */
+    int64_t rows, ld;  /* table rows, elements from one row to the next */
+    int64_t n_tokens, n_bags;
+    float scale;
+    int32_t reserved;
+    const void* table;
+    const int64_t* tokens;
+    const int64_t* offsets; /* n_bags + 1, or NULL */
+    const float* weights;   /* n_tokens, or NULL for ones */
+    void* out;              /* n_bags rows of dim */
+    int64_t out_ld;
+    float* inv_counts;      /* n_bags; mean only, may be NULL: 1 / c_i for the gradient */
+    void* workspace;
+    int64_t workspace_bytes;
+} hanns_embed_bags_t;
+int64_t hanns_gpu_embed_bags_workspace_bytes(const hanns_embed_bags_t* bags);
+int32_t hanns_gpu_embed_bags_device(const hanns_embed_bags_t* bags, void* stream);
+/* Gradients from grad (n_bags rows of dim, out_dtype, grad_ld elements apart): d_table (may be
+ * NULL; rows x dim of the table's type, every row written) and d_weights (may be NULL;
+ * n_tokens, zero for positions that do not count).  A token's terms are added in the order
+ * of its positions: results do not change from run to run.  `out` is not read; a mean needs
+ * the forward call's inv_counts; table may be NULL when d_weights is. */
+int64_t hanns_gpu_embed_bags_grad_workspace_bytes(const hanns_embed_bags_t* bags);
+int32_t hanns_gpu_embed_bags_grad_device(const hanns_embed_bags_t* bags, const void* grad,
+                                         int64_t grad_ld, void* d_table, int64_t d_table_ld,
+                                         float* d_weights, void* stream);
+
+/* Per row of logits: the log probability of tokens[i] under softmax(logits / temperature),
+ * the entropy, and the `top` most likely tokens with their log probabilities (larger logit
+ * first, ties to the lower token).  A logit of -inf is a masked token.  A token outside
+ * [0, vocab) gives 0 (and no gradient).  A row of -inf alone gives -inf, entropy 0 and no
+ * alternatives; fewer than `top` unmasked logits are padded with (-1, -inf).  A row that
+ * holds NaN or +inf gives NaN and tokens -1. */
+typedef struct {
+    int32_t dtype;
+    int32_t top;       /* 0 .. 32 */
+    int64_t n, vocab, ld;
+    float temperature; /* > 0 */
+    int32_t reserved;
+    const void* logits;
+    const int64_t* tokens;
+    float* logprobs;       /* n */
+    float* entropy;        /* n */
+    int64_t* top_tokens;   /* n x top */
+    float* top_logprobs;   /* n x top */
+    float* stats;          /* n x 4, 16-byte aligned; may be NULL unless a call below follows */
+} hanns_token_logprobs_t;
+int32_t hanns_gpu_token_logprobs_device(const hanns_token_logprobs_t* t, void* stream);
+/* Gradient of the logits from those of logprobs (n), entropy (n) and top_logprobs (n x top);
+ * each may be NULL.  Reads logits, tokens, stats and top_tokens as the forward call left them. */
+int32_t hanns_gpu_token_logprobs_grad_device(const hanns_token_logprobs_t* t,
+                                             const float* g_logprobs, const float* g_entropy,
+                                             const float* g_top, void* d_logits, int64_t d_ld,
+                                             void* stream);
+/* After hanns_gpu_token_logprobs_device with stats: turns its outputs, in place, into those of
+ * (1 - weight) * model + weight * neighbours, where the neighbours' distribution gives the
+ * token d_values[id] of each found id (n x k ids and distances as a search returns them) the
+ * share softmax(-distance / knn_temperature).  A neighbour counts when its id is in
+ * [0, n_values), its distance is finite and its token is in the vocabulary and not masked; a
+ * row without one keeps the model's outputs, and so does an empty or undefined row. */
+int32_t hanns_gpu_neighbour_logprobs_device(const hanns_token_logprobs_t* t, const int64_t* d_ids,
+                                            const float* d_distances, int32_t k,
+                                            const int64_t* d_values, int64_t n_values,
+                                            float weight, float knn_temperature, void* stream);
 
 #ifdef __cplusplus
 }
