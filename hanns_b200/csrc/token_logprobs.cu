@@ -8,10 +8,12 @@
 //   gradient:  dx_v = [ -p_v (gl + sum gk + gH (ln p_v + H)) + gl [v = t] + sum gk [v = id_k] ] / T
 //
 // logprobs_kernel reads the logits once: running maximum, sum and weighted sum per thread
-// (rescaled when the maximum grows), and the alternatives by a threshold that a first look at
-// the row sets, so that the few elements above it go to a buffer in shared memory.  A row is
-// one block's, or a cluster's when there are few rows: each block of the cluster then takes a
-// share of the columns and the first one joins them over distributed shared memory.
+// (rescaled when the maximum grows).  Exponents are in powers of two, y = x c - R with
+// c = log2(e) / T and the reference R = m c as f32 rounds it: any R serves, since the same one
+// is taken off again, and y then has a single rounding.  The alternatives come from a threshold
+// that a first look at the row sets; the few vectors above it go to a buffer in shared memory.
+// A row is one block's, or a cluster's when there are few rows: each block of the cluster then
+// takes a share of the columns and the first one joins them over distributed shared memory.
 //
 // neighbours_kernel mixes in the tokens of a search's neighbours:
 //   w = softmax(-distance / tau),  p_v = (1 - l) q_v + l sum of w_j over neighbours j with token v
@@ -20,8 +22,8 @@
 // and the entropy differs from q's in the neighbours' terms and the factor (1 - l).
 #include <cooperative_groups.h>
 
+#include <algorithm>
 #include <cmath>
-#include <limits>
 
 #include "operators.cuh"
 
@@ -30,10 +32,10 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kMaxThreads = 256;
+constexpr int kMaxThreads = 128;
 constexpr int kUnroll = 4;
 constexpr int kMaxTop = 32;
-constexpr int kCap = 1024;       // buffered candidates of a block
+constexpr int kCap = 1024;       // buffered candidate vectors of a block
 constexpr int kMaxCluster = 8;
 constexpr int kMaxNeighbours = 1024;
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.69314718f;
@@ -79,117 +81,300 @@ __device__ __forceinline__ uint64_t cand_key(float x, int32_t col) {
 __device__ __forceinline__ float key_logit(uint64_t k) { return key_to_float((uint32_t)(k >> 32)); }
 __device__ __forceinline__ int32_t key_col(uint64_t k) { return (int32_t)(0xffffffffu - (uint32_t)k); }
 
-// A row's elements as 16-byte vectors from the 16-byte boundary at or before its first one;
-// the vectors that the row does not fill are read element by element, -inf outside the row.
+// A row's elements as 16-byte vectors, numbered from the 16-byte boundary at or before its first
+// one.  Those that the row fills are body[0 .. n); the vector before them and the one behind
+// them may be filled in part and are read element by element, -inf outside the row.
 template <class T>
 struct RowView {
     static constexpr int VE = 16 / sizeof(T);
     const T* row;
-    int lead, vocab;
+    const Pack<T, VE>* body;
+    int lead, vocab, n;
     __device__ __forceinline__ RowView(const T* r, int v)
-        : row(r), lead((int)(((uintptr_t)r & 15) / sizeof(T))), vocab(v) {}
-    __device__ __forceinline__ int vectors() const { return (int)(((int64_t)lead + vocab + VE - 1) / VE); }
-    __device__ __forceinline__ int64_t first(int i) const { return (int64_t)i * VE - lead; }
-    __device__ __forceinline__ Pack<T, VE> load(int i) const {
+        : row(r), lead((int)(((uintptr_t)r & 15) / sizeof(T))), vocab(v) {
+        const int head = lead ? min(VE - lead, vocab) : 0;
+        body = reinterpret_cast<const Pack<T, VE>*>(row + head);
+        n = (vocab - head) / VE;
+    }
+    __device__ __forceinline__ int skipped() const { return lead ? 1 : 0; }  // vectors before the body
+    __device__ __forceinline__ int64_t first(int64_t i) const { return i * VE - lead; }
+    __device__ __forceinline__ Pack<T, VE> edge(int64_t i) const {
         const int64_t e = first(i);
-        if (e >= 0 && e + VE <= vocab) return load_pack<T, VE>(row + e);
         Pack<T, VE> p;
 #pragma unroll
         for (int k = 0; k < VE; ++k)
             p.v[k] = e + k >= 0 && e + k < vocab ? row[e + k] : from_f32<T>(-INFINITY);
         return p;
     }
-};
-
-// Sum of 2^y and of 2^y y, y = (x - m) c.
-struct Running {
-    float m = -INFINITY, s = 0.0f, u = 0.0f;
-    __device__ __forceinline__ void grow(float nm, float c) {
-        const float d = fmaxf((m - nm) * c, kLowest), f = ex2(d);
-        u = f * fmaf(d, s, u);
-        s *= f;
-        m = nm;
+    __device__ __forceinline__ Pack<T, VE> load(int64_t i) const {
+        const int64_t j = i - skipped();
+        return j >= 0 && j < n ? body[j] : edge(i);
     }
+    // all vectors, the partial ones among them
+    __device__ __forceinline__ int vectors() const { return (int)(((int64_t)lead + vocab + VE - 1) / VE); }
 };
 
+// Two 16-bit elements in a word: their f32, and the larger of two words' elements (`max_pairs`
+// keeps a NaN, `raise_pairs` drops it).
+template <class T> __device__ __forceinline__ float2 pair_f32(uint32_t w);
+template <> __device__ __forceinline__ float2 pair_f32<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <> __device__ __forceinline__ float2 pair_f32<__half>(uint32_t w) {
+    return __half22float2(*reinterpret_cast<__half2*>(&w));
+}
+template <class T> __device__ __forceinline__ uint32_t max_pairs(uint32_t a, uint32_t b);
+template <> __device__ __forceinline__ uint32_t max_pairs<__nv_bfloat16>(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template <> __device__ __forceinline__ uint32_t max_pairs<__half>(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template <class T> __device__ __forceinline__ uint32_t raise_pairs(uint32_t a, uint32_t b);
+template <> __device__ __forceinline__ uint32_t raise_pairs<__nv_bfloat16>(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template <> __device__ __forceinline__ uint32_t raise_pairs<__half>(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
 template <class T>
-__device__ __forceinline__ float pack_max(const Pack<T, RowView<T>::VE>& p) {
-    float v = to_f32(p.v[0]);
+__device__ __forceinline__ uint4 words(const Pack<T, 8>& p) {
+    return *reinterpret_cast<const uint4*>(&p);
+}
+
+// 16-bit elements are raised to `floor` before their exponent, two per instruction, so that a
+// masked -inf has a finite y (2^y y is then 0 and not NaN).  A row whose maximum is not well
+// above the floor is summed again from its differences (see row_needs_differences).
+template <class T> __device__ __forceinline__ float floor_of();
+template <> __device__ __forceinline__ float floor_of<float>() { return -INFINITY; }
+template <> __device__ __forceinline__ float floor_of<__half>() { return -65504.0f; }
+template <> __device__ __forceinline__ float floor_of<__nv_bfloat16>() { return -0x1p100f; }
+template <class T> __device__ __forceinline__ uint32_t floor_pair();  // the same, twice in a word
+template <> __device__ __forceinline__ uint32_t floor_pair<__half>() { return 0xfbfffbffu; }
+template <> __device__ __forceinline__ uint32_t floor_pair<__nv_bfloat16>() { return 0xf180f180u; }
+
+// y of a vector's elements against the reference R, as pairs.
+template <class T>
+__device__ __forceinline__ void exponents(const Pack<T, 8>& p, float c, float ref, float2 (&y)[4]) {
+    const uint4 w = words(p);
+    const float2 c2 = make_float2(c, c), r2 = make_float2(-ref, -ref);
+    y[0] = fma2_rn(pair_f32<T>(raise_pairs<T>(w.x, floor_pair<T>())), c2, r2);
+    y[1] = fma2_rn(pair_f32<T>(raise_pairs<T>(w.y, floor_pair<T>())), c2, r2);
+    y[2] = fma2_rn(pair_f32<T>(raise_pairs<T>(w.z, floor_pair<T>())), c2, r2);
+    y[3] = fma2_rn(pair_f32<T>(raise_pairs<T>(w.w, floor_pair<T>())), c2, r2);
+}
+__device__ __forceinline__ void exponents(const Pack<float, 4>& p, float c, float ref, float2 (&y)[2]) {
 #pragma unroll
-    for (int k = 1; k < RowView<T>::VE; ++k) v = max_nan(v, to_f32(p.v[k]));
+    for (int i = 0; i < 2; ++i) {
+        y[i] = fma2_rn(make_float2(p.v[2 * i], p.v[2 * i + 1]), make_float2(c, c), make_float2(-ref, -ref));
+        y[i].x = fmaxf(y[i].x, kLowest);
+        y[i].y = fmaxf(y[i].y, kLowest);
+    }
+}
+
+constexpr float kNoRef = -1e37f;  // below every reference that is used
+
+// Largest element, NaN if there is one.
+__device__ __forceinline__ float pack_max(const Pack<float, 4>& p) {
+    return max_nan(max_nan(p.v[0], p.v[1]), max_nan(p.v[2], p.v[3]));
+}
+template <class T>
+__device__ __forceinline__ uint32_t pair_max(const Pack<T, 8>& p) {
+    const uint4 w = words(p);
+    return max_pairs<T>(max_pairs<T>(w.x, w.y), max_pairs<T>(w.z, w.w));
+}
+template <class T>
+__device__ __forceinline__ float pack_max(const Pack<T, 8>& p) {
+    const float2 v = pair_f32<T>(pair_max(p));
+    return max_nan(v.x, v.y);
+}
+// Of several vectors.
+template <int N>
+__device__ __forceinline__ float packs_max(const Pack<float, 4> (&p)[N]) {
+    float v = pack_max(p[0]);
+#pragma unroll
+    for (int q = 1; q < N; ++q) v = max_nan(v, pack_max(p[q]));
     return v;
 }
+template <class T, int N>
+__device__ __forceinline__ float packs_max(const Pack<T, 8> (&p)[N]) {
+    uint32_t w = pair_max(p[0]);
+#pragma unroll
+    for (int q = 1; q < N; ++q) w = max_pairs<T>(w, pair_max(p[q]));
+    const float2 v = pair_f32<T>(w);
+    return max_nan(v.x, v.y);
+}
 
-struct Shared {
-    uint64_t buf[kCap];
-    uint64_t best[kMaxTop];  // this block's alternatives, best first
-    uint32_t hist[256];
-    float red[3][kMaxThreads / 32];
-    uint32_t warp_key[kMaxThreads / 32];
-    int count;      // candidates offered (may pass kCap: then some were dropped)
-    int dropped;
-    uint64_t low;   // fallback: every key from here on is collected
-    float m, s, u;  // of this block's columns
+// f (u + d s), f s for the factor f = 2^d that moves sums from one reference to another.
+__device__ __forceinline__ void rescale(float d, float& s, float& u) {
+    d = fmaxf(d, kLowest);
+    const float f = ex2(d);
+    u = f * fmaf(d, s, u);
+    s *= f;
+}
+
+// Sums of 2^y and of 2^y y of one thread, two of each so that pairs add up in one instruction.
+template <class T>
+struct Running {
+    float m = -INFINITY, ref;
+    float2 s = make_float2(0.0f, 0.0f), u = make_float2(0.0f, 0.0f);
+    // masked elements before the first live one count as 2^0 against the floor, which a row's
+    // maximum far above it makes nothing of
+    __device__ __forceinline__ explicit Running(float c) : ref(sizeof(T) == 2 ? floor_of<T>() * c : kNoRef) {}
+    // before elements of maximum vm are added
+    __device__ __forceinline__ void reach(float vm, float c) {
+        if (!(vm <= m)) {
+            m = max_nan(vm, m);
+            const float to = sizeof(T) == 2 ? fmaxf(m, floor_of<T>()) * c : fmaxf(m * c, kNoRef), d = ref - to;
+            rescale(d, s.x, u.x);
+            rescale(d, s.y, u.y);
+            ref = to;
+        }
+    }
+    __device__ __forceinline__ void add(const Pack<T, RowView<T>::VE>& p, float c) {
+        constexpr int N = RowView<T>::VE / 2;
+        float2 y[N];
+        exponents(p, c, ref, y);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float2 e = make_float2(ex2(y[i].x), ex2(y[i].y));
+            s = add2_rn(s, e);
+            u = fma2_rn(e, y[i], u);
+        }
+    }
 };
 
-__device__ __forceinline__ void offer(Shared& sh, uint64_t key) {
-    const int at = atomicAdd(&sh.count, 1);
-    if (at < kCap) sh.buf[at] = key;
+// Rows for which y = x c - R is not good enough: the reference or the floor overflows, or
+// masked elements at the floor would count (a maximum near the type's lowest value, a very
+// high or low temperature).  They are read again and summed from (x - m) c.
+template <class T>
+__device__ __forceinline__ bool row_needs_differences(float m, float c) {
+    bool bad = !(fabsf(m * c) < -kNoRef);
+    if (sizeof(T) == 2) bad = bad || !(floor_of<T>() * c > kNoRef) || !((floor_of<T>() - m) * c < -150.0f);
+    return bad;
 }
 
-// best[0 .. top) = the largest of the first n buffered keys (all different), 0 behind them.
-__device__ void rank_select(Shared& sh, int n, int top) {
-    for (int i = threadIdx.x; i < top; i += blockDim.x) sh.best[i] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-        const uint64_t k = sh.buf[i];
+// Buffers in shared memory from which the threads of a group (a block, or a warp) choose.
+struct Choice {
+    uint64_t* buf;   // candidate vectors: order of the maximum, then the lower vector
+    int cap;         // a warp's holds every vector of its row; a block's may drop some
+    uint64_t* elem;  // elements of the best vectors, kMaxTop * 8
+    uint64_t* best;  // the alternatives, best first, kMaxTop
+    int* count;      // candidates offered (may pass cap: then some were dropped)
+    __device__ __forceinline__ void offer(uint64_t key) const {
+        const int at = atomicAdd(count, 1);
+        if (at < cap) buf[at] = key;
+    }
+};
+struct BlockGroup {
+    static __device__ __forceinline__ int rank() { return threadIdx.x; }
+    static __device__ __forceinline__ int size() { return blockDim.x; }
+    static __device__ __forceinline__ void sync() { __syncthreads(); }
+};
+struct WarpGroup {
+    static __device__ __forceinline__ int rank() { return threadIdx.x & 31; }
+    static __device__ __forceinline__ int size() { return 32; }
+    static __device__ __forceinline__ void sync() { __syncwarp(); }
+};
+
+// out[0 .. top) = the largest of n different keys, 0 behind them.  Needs a barrier before,
+// ends with one.
+template <class Group>
+__device__ __forceinline__ void rank_select(const uint64_t* keys, int n, uint64_t* out, int top) {
+    for (int i = Group::rank(); i < n; i += Group::size()) {
+        const uint64_t k = keys[i];
         int rank = 0;
-        for (int j = 0; j < n; ++j) rank += sh.buf[j] > k;
-        if (rank < top) sh.best[rank] = k;
+        for (int j = 0; j < n; ++j) rank += keys[j] > k;
+        if (rank < top) out[rank] = k;
     }
-    __syncthreads();
+    for (int i = n + Group::rank(); i < top; i += Group::size()) out[i] = 0;
+    Group::sync();
 }
 
-// Lower bound of the row's `top`-th logit from each thread's first maximum: the smallest over
-// the warps of the warp's ceil(top / warps)-th largest maximum.
-__device__ float first_threshold(Shared& sh, float vm, int top) {
-    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
-    uint32_t key = vm != vm ? 0xffffffffu : total_order_key(vm), found = 0;
-    for (int r = (top + warps - 1) / warps; r > 0; --r) {
-        found = __reduce_max_sync(0xffffffffu, key);
-        const uint32_t who = __ballot_sync(0xffffffffu, key == found);
-        if (lane == __ffs(who) - 1) key = 0;
+// This lane's key's place among the warp's (ties by lane).
+__device__ __forceinline__ int warp_rank(uint32_t key) {
+    const int lane = threadIdx.x & 31;
+    int rank = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+        const uint32_t o = __shfl_sync(0xffffffffu, key, j);
+        rank += o > key || (o == key && j < lane);
     }
-    if (lane == 0) sh.warp_key[threadIdx.x >> 5] = found;
-    __syncthreads();
-    uint32_t low = sh.warp_key[0];
-    for (int w = 1; w < warps; ++w) low = min(low, sh.warp_key[w]);
+    return rank;
+}
+__device__ __forceinline__ uint32_t max_key(float vm) { return vm != vm ? 0xffffffffu : total_order_key(vm); }
+// The `top`-th largest of the lanes' keys, as a logit.
+__device__ __forceinline__ float warp_threshold(uint32_t key, int top) {
+    const int at = __ffs(__ballot_sync(0xffffffffu, warp_rank(key) == top - 1)) - 1;
+    const uint32_t low = __shfl_sync(0xffffffffu, key, at);
     return low <= kKeyMinusInf ? -INFINITY : key_to_float(low);
 }
 
-// Keeps the best of the buffer when it has grown and returns the new threshold.
-__device__ float refine(Shared& sh, int top, float thr) {
-    __syncthreads();
-    const int offered = sh.count, n = min(offered, kCap);
-    __syncthreads();  // every thread has read the count before the first new candidate
-    if (n <= 2 * top + 32) return thr;
-    rank_select(sh, n, top);
-    for (int i = threadIdx.x; i < top; i += blockDim.x) sh.buf[i] = sh.best[i];
-    if (threadIdx.x == 0) {
-        if (offered > kCap) sh.dropped = 1;
-        sh.count = top;
+// best[] from the buffered vectors: the `top` best vectors hold the `top` best elements (each
+// vector before an element's own has an element before it).  Needs a barrier before, ends
+// with one.
+template <class Group, class T>
+__device__ void select_elements(const Choice& ch, const RowView<T>& view, int top) {
+    constexpr int VE = RowView<T>::VE;
+    rank_select<Group>(ch.buf, min(*ch.count, ch.cap), ch.best, top);
+    const uint64_t least = ch.best[top - 1];  // as many elements as this vector's maximum are no worse
+    const float bound = least ? key_logit(least) : -INFINITY;
+    if (Group::rank() == 0) *ch.count = 0;
+    Group::sync();
+    for (int i = Group::rank(); i < top * VE; i += Group::size()) {
+        const uint64_t v = ch.best[i / VE];
+        const int64_t e = v ? view.first(key_col(v)) + i % VE : -1;
+        if (e < 0 || e >= view.vocab) continue;
+        const float x = to_f32(view.row[e]);
+        if (x > -INFINITY && x >= bound) ch.elem[atomicAdd(ch.count, 1)] = cand_key(x, (int32_t)e);
     }
-    __syncthreads();
-    return fmaxf(thr, key_logit(sh.buf[top - 1]));
+    Group::sync();
+    rank_select<Group>(ch.elem, *ch.count, ch.best, top);
 }
 
-// Candidates were dropped (a row that climbs, or ties by the thousand): find by counting key
-// bytes, highest first, a bound that at least `top` and at most kCap keys reach, and collect
-// those.  Reads the columns up to nine times.
+struct Shared {
+    uint64_t buf[kCap], elem[kMaxTop * 8], best[kMaxTop];
+    uint32_t hist[256];
+    float wm[kMaxThreads / 32], wr[kMaxThreads / 32], ws[kMaxThreads / 32], wu[kMaxThreads / 32];
+    uint32_t lead[32];       // maxima of groups of threads
+    float thr;
+    int count;
+    float m, ref, s, u;      // of this block's columns
+    __device__ __forceinline__ Choice choice() { return Choice{buf, kCap, elem, best, &count}; }
+};
+
+// Lower bound of the row's `top`-th logit: the `top`-th of the 32 maxima that groups of threads
+// have in their columns.
+__device__ float block_threshold(Shared& sh, float vm, int top) {
+    constexpr int kGroup = kMaxThreads / 32;
+    uint32_t key = max_key(vm);
+#pragma unroll
+    for (int d = 1; d < kGroup; d <<= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, d));
+    if (threadIdx.x % kGroup == 0) sh.lead[threadIdx.x / kGroup] = key;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const float thr = warp_threshold(sh.lead[threadIdx.x], top);
+        if (threadIdx.x == 0) sh.thr = thr;
+    }
+    __syncthreads();
+    return sh.thr;
+}
+
+// Candidates were dropped (ties by the thousand): find by counting key
+// bytes, highest first, a bound that at least `top` and at most kCap elements reach, collect
+// those and take the best.  Reads the columns up to nine times.
 template <class T>
-__device__ void collect_again(Shared& sh, const RowView<T>& view, int v0, int v1, int top) {
+__device__ void select_again(Shared& sh, const RowView<T>& view, int v0, int v1, int top) {
     const int64_t e0 = max((int64_t)0, view.first(v0)), e1 = min((int64_t)view.vocab, view.first(v1));
-    uint64_t prefix = 0;
+    uint64_t prefix = 0, low = 0;
     int need = top;
     for (int byte = 7; byte >= 0; --byte) {
         __syncthreads();
@@ -207,44 +392,52 @@ __device__ void collect_again(Shared& sh, const RowView<T>& view, int v0, int v1
         while (b > 0 && above + (int)sh.hist[b] < need) above += sh.hist[b--];
         const int reach = top - need + above + (int)sh.hist[b];
         prefix = (prefix << 8) | (uint64_t)b;
-        if (threadIdx.x == 0) sh.low = prefix << (8 * byte);
+        low = prefix << (8 * byte);
         if (reach <= kCap) break;
         need -= above;
     }
     __syncthreads();
-    const uint64_t low = sh.low;
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
     for (int64_t e = e0 + threadIdx.x; e < e1; e += blockDim.x) {
         const float x = to_f32(view.row[e]);
         if (!(x > -INFINITY)) continue;
         const uint64_t k = cand_key(x, (int32_t)e);
-        if (k >= low) offer(sh, k);
+        if (k >= low) sh.choice().offer(k);
     }
-}
-
-__device__ __forceinline__ float block_reduce(Shared& sh, int slot, float v, bool is_max) {
-#pragma unroll
-    for (int d = 16; d; d >>= 1) {
-        const float o = __shfl_xor_sync(0xffffffffu, v, d);
-        v = is_max ? max_nan(v, o) : v + o;
-    }
-    if ((threadIdx.x & 31) == 0) sh.red[slot][threadIdx.x >> 5] = v;
     __syncthreads();
-    v = sh.red[slot][0];
-    for (int w = 1; w < (int)(blockDim.x >> 5); ++w) v = is_max ? max_nan(v, sh.red[slot][w]) : v + sh.red[slot][w];
-    return v;
+    rank_select<BlockGroup>(sh.buf, min(sh.count, kCap), sh.best, top);
 }
 
-// What the columns' sums become against another maximum (an empty or undefined one: nothing).
-__device__ __forceinline__ void rescale(float m, float& s, float& u, float to, float c) {
-    const float d = fmaxf((m - to) * c, kLowest), f = ex2(d);
-    u = f * fmaf(d, s, u);
-    s *= f;
+// A row's outputs from its maximum, reference and sums.
+template <class Group>
+__device__ __forceinline__ void write_row(const ProbArgs& a, int64_t r, int64_t token, float x_t, float m, float ref, float s,
+                                          float u, bool differences, const uint64_t* best) {
+    const bool empty = m == -INFINITY, undefined = !(m < INFINITY);
+    // the sum of e^((x - m) / T): the reference is m c but for f32's rounding of it
+    const float s_m = differences ? s : s * exp2f(-fmaf(m, a.c, -ref)), log_s = logf(s_m);
+    if (Group::rank() == 0) {
+        float lp = 0.0f, h = 0.0f;
+        if (undefined) {
+            lp = h = NAN;
+        } else {
+            if (!empty) h = fmaxf(logf(s) - __fdiv_rn(u, s) * kLn2, 0.0f);
+            if ((uint64_t)token < (uint64_t)a.vocab) lp = empty ? -INFINITY : log_prob(x_t, m, a.inv_t, log_s);
+        }
+        a.logprobs[r] = lp;
+        a.entropy[r] = h;
+        if (a.stats)
+            a.stats[r] = make_float4(empty ? 0.0f : m, empty ? 1.0f : s_m, h, undefined ? NAN : empty ? 0.0f : 1.0f);
+    }
+    for (int i = Group::rank(); i < a.top; i += Group::size()) {
+        const uint64_t k = undefined ? 0 : best[i];
+        a.top_tokens[r * a.top + i] = k ? key_col(k) : -1;
+        a.top_logprobs[r * a.top + i] = undefined ? NAN : k ? log_prob(key_logit(k), m, a.inv_t, log_s) : -INFINITY;
+    }
 }
 
 template <class T, bool Top>
-__global__ void __launch_bounds__(kMaxThreads) logprobs_kernel(ProbArgs a) {
+__global__ void __launch_bounds__(kMaxThreads, 8) logprobs_kernel(ProbArgs a) {
     constexpr int VE = RowView<T>::VE;
     __shared__ Shared sh;
     cg::cluster_group cluster = cg::this_cluster();
@@ -260,126 +453,264 @@ __global__ void __launch_bounds__(kMaxThreads) logprobs_kernel(ProbArgs a) {
         token = a.tokens[r];
         if ((uint64_t)token < (uint64_t)a.vocab) x_t = to_f32(row[token]);
     }
-    if (threadIdx.x == 0) {
-        sh.count = 0;
-        sh.dropped = 0;
-    }
-    __syncthreads();
+    if (threadIdx.x == 0) sh.count = 0;
 
-    Running run;
-    float thr = -INFINITY;
+    Running<T> run(a.c);
+    float best = -INFINITY, second = -INFINITY, third = -INFINITY;  // largest maxima of this thread's rounds
+    int best_round = 0, second_round = 0;
     const int step = blockDim.x * kUnroll;
-    int round = 0, look = 2;
-    for (int base = v0; base < v1; base += step, ++round) {
+    // this block's vectors of the body, in rounds of kUnroll per thread
+    const int b0 = max(0, v0 - view.skipped()), b1 = min(view.n, v1 - view.skipped());
+    int round = 0;
+    for (int base = b0; base < b1; base += step, ++round) {
         Pack<T, VE> p[kUnroll];
-        float vm[kUnroll];
+        const Pack<T, VE>* src = view.body + base + threadIdx.x;
+        if (base + step <= b1) {
 #pragma unroll
-        for (int q = 0; q < kUnroll; ++q) {
-            const int i = base + q * blockDim.x + threadIdx.x;
-            if (i < v1) {
-                p[q] = view.load(i);
-            } else {
+            for (int q = 0; q < kUnroll; ++q) p[q] = src[q * blockDim.x];
+        } else {
 #pragma unroll
-                for (int k = 0; k < VE; ++k) p[q].v[k] = from_f32<T>(-INFINITY);
-            }
-        }
+            for (int q = 0; q < kUnroll; ++q) {
+                if (base + q * (int)blockDim.x + (int)threadIdx.x < b1) {
+                    p[q] = src[q * blockDim.x];
+                } else {
 #pragma unroll
-        for (int q = 0; q < kUnroll; ++q) vm[q] = pack_max<T>(p[q]);
-        if (Top) {
-            if (round == 0) {
-                float t = vm[0];
-#pragma unroll
-                for (int q = 1; q < kUnroll; ++q) t = max_nan(t, vm[q]);
-                thr = first_threshold(sh, t, a.top);
-            } else if (round == look) {
-                thr = refine(sh, a.top, thr);
-                look = 2 * look;
-            }
-        }
-#pragma unroll
-        for (int q = 0; q < kUnroll; ++q) {
-            if (!(vm[q] <= run.m)) run.grow(max_nan(vm[q], run.m), a.c);
-#pragma unroll
-            for (int k = 0; k < VE; ++k) {
-                const float y = fmaxf((to_f32(p[q].v[k]) - run.m) * a.c, kLowest), e = ex2(y);
-                run.s += e;
-                run.u = fmaf(e, y, run.u);
-            }
-            if (Top && vm[q] >= thr) {
-                const int64_t e0 = view.first(base + q * blockDim.x + threadIdx.x);
-#pragma unroll
-                for (int k = 0; k < VE; ++k) {
-                    const float x = to_f32(p[q].v[k]);
-                    if (x >= thr && x > -INFINITY) offer(sh, cand_key(x, (int32_t)(e0 + k)));
+                    for (int k = 0; k < VE; ++k) p[q].v[k] = from_f32<T>(-INFINITY);
                 }
             }
         }
+        const float vm = packs_max(p);
+        if (Top) {
+            third = fmaxf(third, fminf(second, vm));
+            if (vm > second) {
+                const bool first = vm > best;
+                second = first ? best : vm;
+                second_round = first ? best_round : round;
+                best = first ? vm : best;
+                best_round = first ? round : best_round;
+            }
+        }
+        run.reach(vm, a.c);
+#pragma unroll
+        for (int q = 0; q < kUnroll; ++q) run.add(p[q], a.c);
+    }
+    // the alternatives' candidates: a thread whose maxima reach the threshold reads those rounds
+    // again; where a third one does, its warp reads all of that thread's rounds
+    float thr = -INFINITY;
+    if (Top) {
+        thr = block_threshold(sh, best, a.top);
+        auto offer_vector = [&](int j) {
+            const float pm = pack_max(view.body[j]);
+            if (pm >= thr && pm > -INFINITY) sh.choice().offer(cand_key(pm, view.skipped() + j));
+        };
+        const bool many = third >= thr && third > -INFINITY;
+        if (!many) {
+            for (int k = 0; k < 2; ++k) {
+                if ((k ? second : best) < thr || (k ? second : best) == -INFINITY) break;
+                const int j = b0 + (k ? second_round : best_round) * step + (int)threadIdx.x;
+#pragma unroll
+                for (int q = 0; q < kUnroll; ++q)
+                    if (j + q * (int)blockDim.x < b1) offer_vector(j + q * (int)blockDim.x);
+            }
+        }
+        for (uint32_t who = __ballot_sync(0xffffffffu, many); who; who &= who - 1) {
+            const int j0 = b0 + (int)(threadIdx.x & ~31u) + __ffs(who) - 1;
+            for (int j = j0 + (int)(threadIdx.x & 31) * (int)blockDim.x; j < b1; j += 32 * (int)blockDim.x) offer_vector(j);
+        }
+    }
+    // the partial vectors at the row's ends
+    if (threadIdx.x < 2) {
+        const int i = threadIdx.x ? view.skipped() + view.n : 0;
+        if ((threadIdx.x || view.skipped()) && i >= v0 && i < v1) {
+            const Pack<T, VE> p = view.edge(i);
+            const float vm = pack_max(p);
+            if (Top && vm >= thr && vm > -INFINITY) sh.choice().offer(cand_key(vm, i));
+            run.reach(vm, a.c);
+            run.add(p, a.c);
+        }
     }
 
-    const float m = block_reduce(sh, 0, run.m, true);
-    rescale(run.m, run.s, run.u, m, a.c);
-    const float s = block_reduce(sh, 1, run.s, false);
-    const float u = block_reduce(sh, 2, run.u, false);
+    // the warp's sums against its largest reference, then the block's
+    float m = run.m, ref = run.ref, s = run.s.x + run.s.y, u = run.u.x + run.u.y;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+        m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+        ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, d));
+    }
+    rescale(run.ref - ref, s, u);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, d);
+        u += __shfl_xor_sync(0xffffffffu, u, d);
+    }
+    const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    if ((threadIdx.x & 31) == 0) {
+        sh.wm[warp] = m;
+        sh.wr[warp] = ref;
+        sh.ws[warp] = s;
+        sh.wu[warp] = u;
+    }
+    __syncthreads();
+    m = sh.wm[0];
+    ref = sh.wr[0];
+    for (int w = 1; w < warps; ++w) {
+        m = max_nan(m, sh.wm[w]);
+        ref = fmaxf(ref, sh.wr[w]);
+    }
+    s = u = 0.0f;
+    for (int w = 0; w < warps; ++w) {
+        float ps = sh.ws[w], pu = sh.wu[w];
+        rescale(sh.wr[w] - ref, ps, pu);
+        s += ps;
+        u += pu;
+    }
     if (threadIdx.x == 0) {
         sh.m = m;
+        sh.ref = ref;
         sh.s = s;
         sh.u = u;
     }
     if (Top) {
-        __syncthreads();
-        if (sh.dropped || sh.count > kCap) collect_again(sh, view, v0, v1, a.top);
-        __syncthreads();
-        rank_select(sh, min(sh.count, kCap), a.top);
+        if (sh.count > kCap) select_again(sh, view, v0, v1, a.top);
+        else select_elements<BlockGroup>(sh.choice(), view, a.top);
     }
-    if (parts > 1) cluster.sync();
+    if (parts > 1) {
+        cluster.sync();
+        for (int q = 0; q < parts; ++q) {
+            const Shared* o = cluster.map_shared_rank(&sh, q);
+            m = q ? max_nan(m, o->m) : o->m;
+            ref = q ? fmaxf(ref, o->ref) : o->ref;
+        }
+    }
+    const bool empty = m == -INFINITY, undefined = !(m < INFINITY);
+    const bool differences = !empty && !undefined && row_needs_differences<T>(m, a.c);
+    if (differences) {
+        s = u = 0.0f;
+        const int64_t e1 = min((int64_t)a.vocab, view.first(v1));
+        for (int64_t e = max((int64_t)0, view.first(v0)) + threadIdx.x; e < e1; e += blockDim.x) {
+            const float y = fmaxf((to_f32(row[e]) - m) * a.c, kLowest), f = ex2(y);
+            s += f;
+            u = fmaf(f, y, u);
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+            s += __shfl_xor_sync(0xffffffffu, s, d);
+            u += __shfl_xor_sync(0xffffffffu, u, d);
+        }
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) {
+            sh.ws[warp] = s;
+            sh.wu[warp] = u;
+        }
+        __syncthreads();
+        s = u = 0.0f;
+        for (int w = 0; w < warps; ++w) {
+            s += sh.ws[w];
+            u += sh.wu[w];
+        }
+        if (threadIdx.x == 0) {
+            sh.s = s;
+            sh.u = u;
+        }
+        if (parts > 1) cluster.sync();
+    }
     if (part == 0) {
-        float M = m, S = s, U = u;
         if (parts > 1) {
-            for (int q = 1; q < parts; ++q) M = max_nan(M, cluster.map_shared_rank(&sh, q)->m);
-            S = U = 0.0f;
+            s = u = 0.0f;
             for (int q = 0; q < parts; ++q) {
                 const Shared* o = cluster.map_shared_rank(&sh, q);
                 float ps = o->s, pu = o->u;
-                rescale(o->m, ps, pu, M, a.c);
-                S += ps;
-                U += pu;
+                if (!differences) rescale(o->ref - ref, ps, pu);
+                s += ps;
+                u += pu;
             }
             if (Top) {
                 if (threadIdx.x == 0) sh.count = 0;
                 __syncthreads();
                 for (int i = threadIdx.x; i < parts * a.top; i += blockDim.x) {
                     const uint64_t k = cluster.map_shared_rank(&sh, i / a.top)->best[i % a.top];
-                    if (k) offer(sh, k);
+                    if (k) sh.elem[atomicAdd(&sh.count, 1)] = k;
                 }
                 __syncthreads();
-                rank_select(sh, sh.count, a.top);
+                rank_select<BlockGroup>(sh.elem, sh.count, sh.best, a.top);
             }
         }
-        const bool empty = M == -INFINITY, undefined = !(M < INFINITY);
-        const float log_s = logf(S);
-        if (threadIdx.x == 0) {
-            float lp = 0.0f, h = 0.0f;
-            if (undefined) {
-                lp = h = NAN;
-            } else {
-                if (!empty) h = fmaxf(log_s - __fdiv_rn(U, S) * kLn2, 0.0f);
-                if ((uint64_t)token < (uint64_t)a.vocab) lp = empty ? -INFINITY : log_prob(x_t, M, a.inv_t, log_s);
-            }
-            a.logprobs[r] = lp;
-            a.entropy[r] = h;
-            if (a.stats)
-                a.stats[r] = make_float4(empty ? 0.0f : M, empty ? 1.0f : S, h, undefined ? NAN : empty ? 0.0f : 1.0f);
-        }
-        if (Top) {
-            for (int i = threadIdx.x; i < a.top; i += blockDim.x) {
-                const uint64_t k = undefined ? 0 : sh.best[i];
-                a.top_tokens[r * a.top + i] = k ? key_col(k) : -1;
-                a.top_logprobs[r * a.top + i] =
-                    undefined ? NAN : k ? log_prob(key_logit(k), M, a.inv_t, log_s) : -INFINITY;
-            }
-        }
+        write_row<BlockGroup>(a, r, token, x_t, m, ref, s, u, differences, sh.best);
     }
     if (parts > 1) cluster.sync();  // the others' shared memory stays until it has been read
+}
+
+// Short rows: a warp takes a row whose vectors (the partial ones among them) fit in its
+// registers, kUnroll a lane, and goes on to another.
+constexpr int kRowVectors = 32 * kUnroll;
+
+template <class T, bool Top>
+__global__ void __launch_bounds__(kMaxThreads, 8) logprobs_rows_kernel(ProbArgs a, int64_t n) {
+    constexpr int VE = RowView<T>::VE, kWarps = kMaxThreads / 32;
+    __shared__ uint64_t buf[kWarps][Top ? kRowVectors : 1], elem[kWarps][Top ? kMaxTop * 8 : 1], top_keys[kWarps][kMaxTop];
+    __shared__ int count[kWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Choice ch{buf[warp], kRowVectors, elem[warp], top_keys[warp], &count[warp]};
+    for (int64_t r = (int64_t)blockIdx.x * kWarps + warp; r < n; r += (int64_t)gridDim.x * kWarps) {
+        const T* row = static_cast<const T*>(a.logits) + r * a.ld;
+        const RowView<T> view(row, a.vocab);
+        const int nvec = view.vectors();
+        Pack<T, VE> p[kUnroll];
+#pragma unroll
+        for (int q = 0; q < kUnroll; ++q) {
+            if (q * 32 + lane < nvec) {
+                p[q] = view.load(q * 32 + lane);
+            } else {
+#pragma unroll
+                for (int k = 0; k < VE; ++k) p[q].v[k] = from_f32<T>(-INFINITY);
+            }
+        }
+        const int64_t token = a.tokens[r];
+        const float x_t = (uint64_t)token < (uint64_t)a.vocab ? to_f32(row[token]) : 0.0f;
+        const float vm = packs_max(p);
+        float m = vm;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+        const bool differences = m > -INFINITY && m < INFINITY && row_needs_differences<T>(m, a.c);
+        Running<T> run(a.c);
+        float s, u;
+        if (!differences) {
+            run.reach(m, a.c);  // nothing added yet: this sets the reference
+#pragma unroll
+            for (int q = 0; q < kUnroll; ++q)
+                if (q * 32 < nvec) run.add(p[q], a.c);
+            s = run.s.x + run.s.y;
+            u = run.u.x + run.u.y;
+        } else {
+            s = u = 0.0f;
+            for (int e = lane; e < a.vocab; e += 32) {
+                const float y = fmaxf((to_f32(row[e]) - m) * a.c, kLowest), f = ex2(y);
+                s += f;
+                u = fmaf(f, y, u);
+            }
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+            s += __shfl_xor_sync(0xffffffffu, s, d);
+            u += __shfl_xor_sync(0xffffffffu, u, d);
+        }
+        if (Top) {
+            if (lane == 0) count[warp] = 0;
+            __syncwarp();
+            const float thr = warp_threshold(max_key(vm), a.top);
+            if (vm >= thr) {
+#pragma unroll
+                for (int q = 0; q < kUnroll; ++q) {
+                    const float pm = pack_max(p[q]);
+                    if (pm >= thr && pm > -INFINITY) ch.offer(cand_key(pm, q * 32 + lane));
+                }
+            }
+            __syncwarp();
+            select_elements<WarpGroup>(ch, view, a.top);
+        }
+        write_row<WarpGroup>(a, r, token, x_t, m, run.ref, s, u, differences, top_keys[warp]);
+        __syncwarp();
+    }
 }
 
 // ---------------------------------------------------------------- gradient
@@ -635,23 +966,25 @@ void check_probs(const hanns_token_logprobs_t* t) {
     require((uintptr_t)t->stats % 16 == 0, "token_logprobs: stats must be 16-byte aligned");
 }
 
-int sm_count() {
-    int dev = 0, n = 0;
-    HANNS_CUDA_OK(cudaGetDevice(&dev));
-    HANNS_CUDA_OK(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
-    return n;
-}
+// The launch rules count the SMs of a B200 (a launch is right on any number).
+constexpr int sm_count() { return 148; }
 
 template <class T, bool Top>
 void launch_probs(const hanns_token_logprobs_t* t, const ProbArgs& a, cudaStream_t s) {
-    const int64_t vectors = (t->vocab + RowView<T>::VE - 1) / RowView<T>::VE + 1;
-    // A cluster's blocks share a row when the rows alone do not give every SM two blocks,
-    // as long as each block still has two rounds of full loads.
+    const int64_t vectors = (t->vocab + RowView<T>::VE - 1) / RowView<T>::VE + 1;  // one more where a row starts inside a vector
+    if (vectors <= kRowVectors) {
+        constexpr int warps = kMaxThreads / 32;
+        const int64_t blocks = std::min<int64_t>((t->n + warps - 1) / warps, 8 * sm_count());
+        logprobs_rows_kernel<T, Top><<<(unsigned)blocks, kMaxThreads, 0, s>>>(a, t->n);
+        HANNS_CUDA_OK(cudaGetLastError());
+        return;
+    }
+    // A cluster's blocks share a row when the rows alone do not give every SM four blocks, as
+    // long as each block still has a round of full loads.
     int parts = 1;
-    const int64_t want = 2 * sm_count();
-    while (parts < kMaxCluster && t->n * parts * 2 <= want && vectors / (parts * 2) >= 2 * kMaxThreads) parts *= 2;
-    int threads = 32;
-    while (threads < kMaxThreads && vectors / parts > (int64_t)threads * kUnroll) threads *= 2;
+    const int64_t want = 4 * sm_count();
+    while (parts < kMaxCluster && t->n * parts * 2 <= want && vectors / (parts * 2) >= kMaxThreads * kUnroll) parts *= 2;
+    const int threads = kMaxThreads;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(t->n * parts));
     cfg.blockDim = dim3((unsigned)threads);

@@ -48,8 +48,10 @@ def _cuda(t, name):
 
 def _ids(t, device, name):
     _on(t, device, name)
-    _need(t.dtype in (torch.int64, torch.int32), f"{name} must be int64 or int32, not {t.dtype}")
-    return t.to(torch.int64).contiguous()
+    if t.dtype != torch.int64:
+        _need(t.dtype == torch.int32, f"{name} must be int64 or int32, not {t.dtype}")
+        t = t.to(torch.int64)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _ptr(t):
@@ -61,41 +63,48 @@ def _rows(t):
     return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+def _run(dev, work):
+    """work(stream) with dev current, on dev's current stream."""
+    if torch.cuda.current_device() == dev.index:
+        return work(torch._C._cuda_getCurrentRawStream(dev.index))
+    with torch.cuda.device(dev):
+        return work(torch._C._cuda_getCurrentRawStream(dev.index))
 
 
-def _workspace(nbytes, device):
+def _workspace(nbytes, device, b):
     if nbytes < 0:
         raise ValueError(f"embed_bags: {L.last_error()}")
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    if not nbytes:
+        return None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    b.workspace, b.workspace_bytes = ws.data_ptr(), nbytes
+    return ws
 
 
 # ---------------------------------------------------------------------------- embed_bags
 def _bags(table, tokens, offsets, weights, scale, mean, out_dtype, inv_counts):
-    b = L.EmbedBags()
-    b.dtype, b.out_dtype = _DTYPES[table.dtype], _DTYPES[out_dtype]
-    b.rows, b.dim = table.shape
-    b.ld, b.mean, b.scale = table.stride(0), int(mean), scale
-    b.n_tokens = tokens.numel()
-    b.n_bags = b.n_tokens if offsets is None else offsets.numel() - 1
-    b.table, b.tokens, b.offsets = _ptr(table), _ptr(tokens), _ptr(offsets)
-    b.weights, b.inv_counts = _ptr(weights), _ptr(inv_counts)
-    return b
+    rows, dim = table.shape
+    n = tokens.shape[0]
+    return L.EmbedBags(_DTYPES[table.dtype], _DTYPES[out_dtype], dim, int(mean), rows, table.stride(0), n,
+                       n if offsets is None else offsets.shape[0] - 1, scale, 0, table.data_ptr(),
+                       tokens.data_ptr(), _ptr(offsets), _ptr(weights), None, 0, _ptr(inv_counts), None, 0)
 
 
 def _embed_bags(table, tokens, offsets, weights, scale, mean, out_dtype, keep):
     """The vectors, and with `keep` what a mean's gradient needs (1 / c_i)."""
     dev = table.device
-    n_bags = tokens.numel() if offsets is None else offsets.numel() - 1
+    n_bags = tokens.shape[0] if offsets is None else offsets.shape[0] - 1
     inv = torch.empty(n_bags, dtype=torch.float32, device=dev) if mean and keep else None
-    out = torch.empty(n_bags, table.shape[1], dtype=out_dtype, device=dev)
+    out = torch.empty((n_bags, table.shape[1]), dtype=out_dtype, device=dev)
     b = _bags(table, tokens, offsets, weights, scale, mean, out_dtype, inv)
-    b.out, b.out_ld = _ptr(out), out.stride(0)
-    with torch.cuda.device(dev):
-        ws = _workspace(L.lib().hanns_gpu_embed_bags_workspace_bytes(C.byref(b)), dev)
-        b.workspace, b.workspace_bytes = _ptr(ws), 0 if ws is None else ws.numel()
-        _check(L.lib().hanns_gpu_embed_bags_device(C.byref(b), _stream(dev)), "embed_bags")
+    b.out, b.out_ld = out.data_ptr(), table.shape[1]
+    lib, ref = L.lib(), C.byref(b)
+
+    def work(stream):
+        ws = _workspace(lib.hanns_gpu_embed_bags_workspace_bytes(ref), dev, b)  # noqa: F841 (kept until enqueued)
+        _check(lib.hanns_gpu_embed_bags_device(ref, stream), "embed_bags")
+
+    _run(dev, work)
     return out, inv
 
 
@@ -125,14 +134,16 @@ def _embed_bags_grad(grad, table, tokens, offsets, weights, inv, scale, mean, ou
     if want_weights:
         d_weights = torch.empty(tokens.numel(), dtype=torch.float32, device=dev)
     b = _bags(table, tokens, offsets, weights, scale, mean, out_dtype, inv)
-    with torch.cuda.device(dev):
-        ws = None
+    lib, ref = L.lib(), C.byref(b)
+
+    def work(stream):
+        ws = None  # noqa: F841 (kept until enqueued)
         if want_table:
-            ws = _workspace(L.lib().hanns_gpu_embed_bags_grad_workspace_bytes(C.byref(b)), dev)
-        b.workspace, b.workspace_bytes = _ptr(ws), 0 if ws is None else ws.numel()
-        _check(L.lib().hanns_gpu_embed_bags_grad_device(
-            C.byref(b), _ptr(grad), grad.stride(0), _ptr(d_table),
-            d_table.stride(0) if want_table else 0, _ptr(d_weights), _stream(dev)), "embed_bags")
+            ws = _workspace(lib.hanns_gpu_embed_bags_grad_workspace_bytes(ref), dev, b)  # noqa: F841
+        _check(lib.hanns_gpu_embed_bags_grad_device(ref, grad.data_ptr(), grad.stride(0), _ptr(d_table), table.shape[1],
+                                                    _ptr(d_weights), stream), "embed_bags")
+
+    _run(dev, work)
     return d_table, d_weights
 
 
@@ -164,7 +175,8 @@ def embed_bags(table, tokens, offsets=None, weights=None, *, scale: float = 1.0,
     tokens = _ids(tokens, dev, "tokens")
     shape = tokens.shape
     if offsets is None:
-        tokens = tokens.reshape(-1)
+        if tokens.dim() != 1:
+            tokens = tokens.reshape(-1)
     else:
         _need(tokens.dim() == 1, "tokens must be one-dimensional when offsets are given")
         offsets = _ids(offsets, dev, "offsets")
@@ -173,15 +185,16 @@ def embed_bags(table, tokens, offsets=None, weights=None, *, scale: float = 1.0,
         _on(weights, dev, "weights")
         _need(weights.dtype == torch.float32, "weights must be float32")
         _need(weights.numel() == tokens.numel(), "weights must have one value per token")
-        weights = weights.reshape(-1).contiguous()
+        if weights.dim() != 1 or not weights.is_contiguous():
+            weights = weights.reshape(-1).contiguous()
     scale = float(scale)
     _need(scale == scale and abs(scale) != float("inf"), "scale must be finite")
     args = _rows(table), tokens, offsets, weights, scale, bool(mean), out_dtype
-    if torch.is_grad_enabled() and (table.requires_grad or weights is not None and weights.requires_grad):
+    if (table.requires_grad or weights is not None and weights.requires_grad) and torch.is_grad_enabled():
         out = _EmbedBags.apply(*args)
     else:
         out, _ = _embed_bags(*args, False)
-    return out.reshape(*shape, table.shape[1]) if offsets is None else out
+    return out.reshape(*shape, table.shape[1]) if offsets is None and len(shape) != 1 else out
 
 
 # ---------------------------------------------------------------------------- token_logprobs
@@ -210,30 +223,31 @@ class Neighbours:
 
 
 def _probs(logits, tokens, top, temperature, out):
-    t = L.TokenLogprobs()
-    t.dtype, t.top, t.temperature = _DTYPES[logits.dtype], top, temperature
-    t.n, t.vocab = logits.shape
-    t.ld = logits.stride(0)
-    t.logits, t.tokens = _ptr(logits), _ptr(tokens)
-    t.logprobs, t.entropy, t.top_tokens, t.top_logprobs, t.stats = (_ptr(o) for o in out)
-    return t
+    n, vocab = logits.shape
+    return L.TokenLogprobs(_DTYPES[logits.dtype], top, n, vocab, logits.stride(0), temperature, 0,
+                           logits.data_ptr(), tokens.data_ptr(), out[0].data_ptr(), out[1].data_ptr(),
+                           out[2].data_ptr(), out[3].data_ptr(), _ptr(out[4]))
 
 
 def _token_logprobs(logits, tokens, top, temperature, near, keep):
     """logprobs, entropy, top tokens, top logprobs and, with `keep`, the rows' statistics."""
     dev, n = logits.device, logits.shape[0]
-    f32 = dict(dtype=torch.float32, device=dev)
-    out = (torch.empty(n, **f32), torch.empty(n, **f32),
-           torch.empty(n, top, dtype=torch.int64, device=dev), torch.empty(n, top, **f32),
-           torch.empty(n, 4, **f32) if keep or near is not None else None)
+    f32 = torch.float32
+    out = (torch.empty(n, dtype=f32, device=dev), torch.empty(n, dtype=f32, device=dev),
+           torch.empty((n, top), dtype=torch.int64, device=dev), torch.empty((n, top), dtype=f32, device=dev),
+           torch.empty((n, 4), dtype=f32, device=dev) if keep or near is not None else None)
     t = _probs(logits, tokens, top, temperature, out)
-    with torch.cuda.device(dev):
-        _check(L.lib().hanns_gpu_token_logprobs_device(C.byref(t), _stream(dev)), "token_logprobs")
+    lib, ref = L.lib(), C.byref(t)
+
+    def work(stream):
+        _check(lib.hanns_gpu_token_logprobs_device(ref, stream), "token_logprobs")
         if near is not None:
             ids, distances, values, weight, knn_temperature = near
-            _check(L.lib().hanns_gpu_neighbour_logprobs_device(
-                C.byref(t), _ptr(ids), _ptr(distances), ids.shape[-1], _ptr(values), values.numel(),
-                weight, knn_temperature, _stream(dev)), "token_logprobs")
+            _check(lib.hanns_gpu_neighbour_logprobs_device(
+                ref, ids.data_ptr(), distances.data_ptr(), ids.shape[-1], values.data_ptr(), values.numel(),
+                weight, knn_temperature, stream), "token_logprobs")
+
+    _run(dev, work)
     return out
 
 
@@ -255,9 +269,8 @@ class _TokenLogprobs(torch.autograd.Function):
         g = [None if x is None else x.to(torch.float32).contiguous() for x in (g_logprobs, g_entropy, g_top)]
         d = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
         t = _probs(logits, tokens, *ctx.args, out)
-        with torch.cuda.device(dev):
-            _check(L.lib().hanns_gpu_token_logprobs_grad_device(
-                C.byref(t), *(_ptr(x) for x in g), _ptr(d), d.stride(0), _stream(dev)), "token_logprobs")
+        _run(dev, lambda stream: _check(L.lib().hanns_gpu_token_logprobs_grad_device(
+            C.byref(t), *(_ptr(x) for x in g), d.data_ptr(), logits.shape[1], stream), "token_logprobs"))
         return d, None, None, None
 
 
@@ -300,10 +313,15 @@ def token_logprobs(logits, tokens, *, top: int = 0, temperature: float = 1.0,
         _need(values.dim() == 1, "neighbours.values must be one-dimensional")
         near = (ids, neighbours.distances.contiguous(), values, float(neighbours.weight),
                 float(neighbours.temperature))
-    args = _rows(logits).reshape(-1, vocab), tokens.reshape(-1), top, temperature
-    if torch.is_grad_enabled() and logits.requires_grad:
-        lp, h, tt, tl = _TokenLogprobs.apply(*args)
+    plain = logits.dim() == 2
+    args = _rows(logits), tokens, top, temperature
+    if not plain:
+        args = args[0].reshape(-1, vocab), tokens.reshape(-1), top, temperature
+    if logits.requires_grad and torch.is_grad_enabled():
+        out = _TokenLogprobs.apply(*args)
     else:
-        lp, h, tt, tl, _ = _token_logprobs(*args, near, False)
+        out = _token_logprobs(*args, near, False)
+    if plain:
+        return TokenLogprobs(*out[:4])
     s = tokens.shape
-    return TokenLogprobs(lp.reshape(s), h.reshape(s), tt.reshape(*s, top), tl.reshape(*s, top))
+    return TokenLogprobs(out[0].reshape(s), out[1].reshape(s), out[2].reshape(*s, top), out[3].reshape(*s, top))
