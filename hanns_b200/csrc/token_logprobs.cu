@@ -34,6 +34,8 @@ namespace cg = cooperative_groups;
 
 constexpr int kMaxThreads = 128;
 constexpr int kUnroll = 4;
+constexpr int kGradThreads = 128, kGradUnroll = 2;
+constexpr int kGradRounds = 8;  // of a block, where there are blocks enough
 constexpr int kMaxTop = 32;
 constexpr int kCap = 1024;       // buffered candidate vectors of a block
 constexpr int kMaxCluster = 8;
@@ -144,6 +146,15 @@ template <> __device__ __forceinline__ uint32_t raise_pairs<__half>(uint32_t a, 
     uint32_t r;
     asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
+}
+template <class T> __device__ __forceinline__ uint32_t pack_pair(float2 v);
+template <> __device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float2 v) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack_pair<__half>(float2 v) {
+    const __half2 h = __floats2half2_rn(v.x, v.y);
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
 template <class T>
 __device__ __forceinline__ uint4 words(const Pack<T, 8>& p) {
@@ -725,82 +736,139 @@ struct GradArgs {
     const float4* stats;
     const float *g_logprobs, *g_entropy, *g_top;
     void* out;
-    int blocks_per_row;
+    int blocks_per_row, span;
 };
 
+// dx_v before its own terms: -p_v (G + gH (ln p_v + H)) / T = 2^y_v (base + slope y_v), where
+// 2^y / s = p and ln p = y ln 2 - ln s.
 struct RowGrad {
-    float m, inv_s, log_s, h, g, gh, c, inv_t;
-    // -p (G + gH (ln p + H)) before 1 / T
+    float m, c, ref, base, slope;
+    // from (x - m) c
     __device__ __forceinline__ float dense(float x) const {
-        const float y = fmaxf((x - m) * c, kLowest), p = ex2(y) * inv_s;
-        return -p * fmaf(gh, fmaf(y, kLn2, h - log_s), g);
+        const float y = fmaxf((x - m) * c, kLowest);
+        return ex2(y) * fmaf(slope, y, base);
     }
 };
 
+// Of a vector; the reference here is m c itself, so y is off by its rounding, which `base` and
+// `slope` take back (they are of the sum against that reference).
+template <class T>
+__device__ __forceinline__ void dense_vector(const RowGrad& g, const Pack<T, 8>& p, Pack<T, 8>& d) {
+    float2 y[4];
+    exponents(p, g.c, g.ref, y);
+    uint32_t* out = reinterpret_cast<uint32_t*>(&d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = fma2_rn(y[i], make_float2(g.slope, g.slope), make_float2(g.base, g.base));
+        const float2 v = mul2_rn(make_float2(ex2(y[i].x), ex2(y[i].y)), f);
+        out[i] = pack_pair<T>(v);
+    }
+}
+__device__ __forceinline__ void dense_vector(const RowGrad& g, const Pack<float, 4>& p, Pack<float, 4>& d) {
+    float2 y[2];
+    exponents(p, g.c, g.ref, y);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float2 f = fma2_rn(y[i], make_float2(g.slope, g.slope), make_float2(g.base, g.base));
+        d.v[2 * i] = ex2(y[i].x) * f.x;
+        d.v[2 * i + 1] = ex2(y[i].y) * f.y;
+    }
+}
+
+// Blocks take `span` vectors of a row each; its first block takes the partial ones at its ends.
 template <class T, bool Wide>
-__global__ void __launch_bounds__(kMaxThreads) logprobs_grad_kernel(GradArgs a) {
+__global__ void __launch_bounds__(kGradThreads, 12) logprobs_grad_kernel(GradArgs a) {
     constexpr int VE = RowView<T>::VE;
     const int64_t r = blockIdx.x / (unsigned)a.blocks_per_row;
-    const int chunk = (int)(blockIdx.x - r * a.blocks_per_row);
+    const int part = (int)(blockIdx.x - r * a.blocks_per_row);
     const T* row = static_cast<const T*>(a.logits) + r * a.ld;
     T* out = static_cast<T*>(a.out) + r * a.out_ld;
+    const RowView<T> view(row, a.vocab);
+    const int b0 = min(view.n, part * a.span), b1 = min(view.n, b0 + a.span);
     const float4 st = a.stats[r];
-    const bool live = st.w == 1.0f;
+    const bool live = st.w == 1.0f, undefined = !(st.w == st.w);
     const int64_t token = a.tokens[r];
     const bool given = (uint64_t)token < (uint64_t)a.vocab;
     const float gl = a.g_logprobs && given ? a.g_logprobs[r] : 0.0f;
-    RowGrad rg;
-    rg.m = st.x;
-    rg.inv_s = __fdiv_rn(1.0f, st.y);
-    rg.log_s = logf(st.y);
-    rg.h = st.z;
-    rg.g = gl;
-    rg.gh = a.g_entropy ? a.g_entropy[r] : 0.0f;
-    rg.c = a.c;
-    rg.inv_t = a.inv_t;
+    const float gh = a.g_entropy ? a.g_entropy[r] : 0.0f;
+    float g = gl;
     if (a.g_top)
         for (int k = 0; k < a.top; ++k)
-            if (a.top_tokens[r * a.top + k] >= 0) rg.g += a.g_top[r * a.top + k];
-    if (!(st.w == st.w)) rg.g = NAN;
-
-    const RowView<T> view(row, a.vocab);
-    const int nvec = view.vectors(), per = kMaxThreads * kUnroll;
-    const int v0 = chunk * per, v1 = min(nvec, v0 + per);
-    Pack<T, VE> p[kUnroll];
-#pragma unroll
-    for (int q = 0; q < kUnroll; ++q) {
-        const int i = v0 + q * kMaxThreads + threadIdx.x;
-        if (i < v1) p[q] = view.load(i);
-    }
-#pragma unroll
-    for (int q = 0; q < kUnroll; ++q) {
-        const int i = v0 + q * kMaxThreads + threadIdx.x;
-        if (i >= v1) continue;
-        Pack<T, VE> d;
-#pragma unroll
-        for (int k = 0; k < VE; ++k) d.v[k] = from_f32<T>(rg.dense(to_f32(p[q].v[k])) * a.inv_t);
-        const int64_t e = view.first(i);
-        if (Wide && e >= 0 && e + VE <= a.vocab) {
-            *reinterpret_cast<Pack<T, VE>*>(out + e) = d;
+            if (a.top_tokens[r * a.top + k] >= 0) g += a.g_top[r * a.top + k];
+    RowGrad rg;
+    rg.m = st.x;
+    rg.c = a.c;
+    rg.ref = st.x * a.c;
+    const float scale = -__fdiv_rn(a.inv_t, st.y);
+    rg.base = scale * (g + gh * (st.z - logf(st.y)));
+    rg.slope = scale * gh * kLn2;
+    if (undefined) rg.base = NAN;
+    if (!live) rg.m = rg.c = 0.0f;  // 2^0 base: NaN, or the zeros of an empty row
+    if (!live && !undefined) rg.base = rg.slope = 0.0f;
+    Pack<T, VE>* wide_out = reinterpret_cast<Pack<T, VE>*>(out + (view.skipped() ? view.first(1) : 0));
+    auto store = [&](int j, const Pack<T, VE>& d) {
+        if (Wide) {
+            wide_out[j] = d;
         } else {
+            const int64_t e = view.first(j + view.skipped());
 #pragma unroll
-            for (int k = 0; k < VE; ++k)
-                if (e + k >= 0 && e + k < a.vocab) out[e + k] = d.v[k];
+            for (int k = 0; k < VE; ++k) out[e + k] = d.v[k];
         }
+    };
+    if (!live || row_needs_differences<T>(st.x, a.c)) {
+        for (int j = b0 + threadIdx.x; j < b1; j += kGradThreads) {
+            const Pack<T, VE> p = view.body[j];
+            Pack<T, VE> d;
+#pragma unroll
+            for (int k = 0; k < VE; ++k) d.v[k] = from_f32<T>(live ? rg.dense(to_f32(p.v[k])) : rg.base);
+            store(j, d);
+        }
+    } else {
+        RowGrad near = rg;  // against the rounded reference: 2^y is larger by 2^rest
+        const float rest = fmaf(rg.m, rg.c, -rg.ref), f = exp2f(-rest);
+        near.base = f * fmaf(-rest, rg.slope, rg.base);
+        near.slope = f * rg.slope;
+        for (int base = b0; base < b1; base += kGradThreads * kGradUnroll) {
+            Pack<T, VE> p[kGradUnroll];
+            const int j = base + threadIdx.x;
+            if (base + kGradThreads * kGradUnroll <= b1) {
+#pragma unroll
+                for (int q = 0; q < kGradUnroll; ++q) p[q] = view.body[j + q * kGradThreads];
+#pragma unroll
+                for (int q = 0; q < kGradUnroll; ++q) {
+                    Pack<T, VE> d;
+                    dense_vector(near, p[q], d);
+                    store(j + q * kGradThreads, d);
+                }
+            } else {
+                for (int i = j; i < b1; i += kGradThreads) {
+                    const Pack<T, VE> v = view.body[i];
+                    Pack<T, VE> d;
+                    dense_vector(near, v, d);
+                    store(i, d);
+                }
+            }
+        }
+    }
+    const int64_t head = view.skipped() ? min((int64_t)a.vocab, view.first(1)) : 0, tail = head + (int64_t)view.n * VE;
+    if (part == 0 && threadIdx.x < 2 * VE) {
+        const int64_t e = (int)threadIdx.x < VE ? (int64_t)threadIdx.x : tail + threadIdx.x - VE;
+        if ((int)threadIdx.x < VE ? e < head : e < a.vocab) out[e] = from_f32<T>(live ? rg.dense(to_f32(row[e])) : rg.base);
     }
     // the given token and the alternatives have terms of their own
     if (!live) return;
     __syncthreads();
-    const int64_t e0 = view.first(v0), e1 = view.first(v1);
-    for (int i = threadIdx.x; i <= a.top; i += kMaxThreads) {
+    const int64_t e0 = head + (int64_t)b0 * VE, e1 = head + (int64_t)b1 * VE;
+    for (int i = threadIdx.x; i <= a.top; i += kGradThreads) {
         if (i > 0 && !a.g_top) break;
         const int64_t v = i == 0 ? token : a.top_tokens[r * a.top + i - 1];
-        if ((uint64_t)v >= (uint64_t)a.vocab || v < e0 || v >= e1) continue;
+        if ((uint64_t)v >= (uint64_t)a.vocab) continue;
+        if (v < head || v >= tail ? part != 0 : v < e0 || v >= e1) continue;
         float own = v == token ? gl : 0.0f;
         if (a.g_top)
             for (int k = 0; k < a.top; ++k)
                 if (a.top_tokens[r * a.top + k] == v) own += a.g_top[r * a.top + k];
-        out[v] = from_f32<T>((own + rg.dense(to_f32(row[v]))) * a.inv_t);
+        out[v] = from_f32<T>(fmaf(own, a.inv_t, rg.dense(to_f32(row[v]))));
     }
 }
 
@@ -999,14 +1067,19 @@ void launch_probs(const hanns_token_logprobs_t* t, const ProbArgs& a, cudaStream
 
 template <class T>
 void launch_grad(const hanns_token_logprobs_t* t, GradArgs a, cudaStream_t s) {
-    const int64_t vectors = (t->vocab + RowView<T>::VE - 1) / RowView<T>::VE + 1;  // one more where a row starts inside a vector
-    a.blocks_per_row = (int)((vectors + kMaxThreads * kUnroll - 1) / (kMaxThreads * kUnroll));
+    const int64_t vectors = (t->vocab + RowView<T>::VE - 1) / RowView<T>::VE;
+    // several rounds to a block, for what a block works out once, unless that leaves SMs idle
+    const int64_t round = kGradThreads * kGradUnroll;
+    int64_t rounds = kGradRounds;
+    while (rounds > 1 && t->n * ((vectors + rounds * round - 1) / (rounds * round)) < 16 * sm_count()) rounds /= 2;
+    a.span = (int)(rounds * round);
+    a.blocks_per_row = (int)((vectors + a.span - 1) / a.span);
     require(t->n * a.blocks_per_row < 0x7fffffff, "token_logprobs: too many elements for one gradient call");
     // wide stores where each output row starts as its logits do within 16 bytes
     const bool wide = ((uintptr_t)a.logits - (uintptr_t)a.out) % 16 == 0 && ((a.ld - a.out_ld) * (int64_t)sizeof(T)) % 16 == 0;
     const unsigned grid = (unsigned)(t->n * a.blocks_per_row);
-    if (wide) logprobs_grad_kernel<T, true><<<grid, kMaxThreads, 0, s>>>(a);
-    else logprobs_grad_kernel<T, false><<<grid, kMaxThreads, 0, s>>>(a);
+    if (wide) logprobs_grad_kernel<T, true><<<grid, kGradThreads, 0, s>>>(a);
+    else logprobs_grad_kernel<T, false><<<grid, kGradThreads, 0, s>>>(a);
     HANNS_CUDA_OK(cudaGetLastError());
 }
 
