@@ -12,11 +12,19 @@
 // does not change from run to run), the segments are the tokens and the matrix is the
 // incoming gradient.  Sums are f32, rounded once to the output's type.
 //
-// A segment of at most `limit` entries is summed by one warp per column tile
-// (segments_kernel).  Longer ones are cut at the multiples of `limit` positions
-// (pieces_kernel writes f32 partial rows) and joined in order (join_kernel), so that one
-// document, or the most frequent token of a batch, does not run on a single warp.
+// A warp sums a segment's rows over a column tile (segments_kernel): its lanes look 32 entries up,
+// put the counted ones side by side in shared memory, and then read several rows at a time, up to
+// four vectors of a row to a lane, without a branch between them.  What an entry, a segment and a
+// warp cost besides is as much as a few vectors' sums, which is why the tiles are wide.  A segment
+// longer than kLimit goes to a list of pieces, each a warp's (pieces_kernel); the last one of a
+// segment to finish adds its pieces up in order, so that one document, or the most frequent token
+// of a batch, does not run on a single warp.
+//
+// The weights' gradient falls out of the table's: the warp that sums token v's gradient rows has
+// E[v]'s tile in registers and takes each row's inner product with it on the way.
 #include <algorithm>
+#include <initializer_list>
+#include <type_traits>
 
 #include "operators.cuh"
 
@@ -24,7 +32,16 @@ namespace hanns {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kUnroll = 4;
+constexpr int kSegmentThreads = 64;   // two warps: a block ends with the longer of two segments
+constexpr int kLimit = 32;            // longest segment of one warp
+constexpr int kPiece = 64;            // least entries of a longer one's pieces
+constexpr int kDots = 8;              // inner products that are reduced together
+// Vectors of a row that a lane takes, rows that it has on the way then, and the blocks of an SM
+// that its registers are kept to (more spill, fewer leave the memory idle).
+constexpr int kMostPacks = 4;
+__host__ __device__ constexpr int rows_ahead(int packs) { return packs == 1 ? 8 : packs == 2 ? 3 : 2; }
+constexpr int blocks_of_sm(int packs, int ve, bool dot) { return packs == 1 ? 14 : ve == 8 ? (dot ? 10 : 16) : dot ? 14 : 18; }
+constexpr int kLookupRows = 8;        // rows of a warp in a lookup
 constexpr int kMaxBinBits = 9, kMaxBins = 1 << kMaxBinBits;
 constexpr int kSortItems = 4, kSortTile = kThreads * kSortItems;
 
@@ -39,11 +56,14 @@ struct TokenEntries {
         row = (uint64_t)t < (uint64_t)rows ? (int)t : -1;
         coef = weights ? weights[j] : 1.0f;
     }
+    __device__ __forceinline__ int position(int64_t j) const { return (int)j; }
 };
 // Entry j of the positions sorted by token.
 struct SortedEntries {
     const int32_t* src;
     const float* coef;
+    const uint32_t* pos;
+    __device__ __forceinline__ int position(int64_t j) const { return (int)pos[j]; }
     __device__ __forceinline__ void get(int64_t j, int& row, float& c) const {
         row = src[j];
         c = coef[j];
@@ -67,31 +87,37 @@ struct BagSegments {
         lo = clamp_pos(offsets[i], 0, n_tokens);
         hi = clamp_pos(offsets[i + 1], lo, n_tokens);
     }
-    // The bag that holds position p, or -1.
-    __device__ __forceinline__ int64_t at(int64_t p) const {
-        if (!offsets) return p;
-        int64_t a = 0, b = n_bags + 1;  // first index whose offset is > p
+    // The number of offsets that are at most p.
+    __device__ __forceinline__ int64_t starts_up_to(int64_t p) const {
+        int64_t a = 0, b = n_bags + 1;
         while (a < b) {
             const int64_t m = (a + b) >> 1;
             if (offsets[m] <= p) a = m + 1;
             else b = m;
         }
-        return a >= 1 && a <= n_bags ? a - 1 : -1;
+        return a;
     }
 };
-// Tokens: runs of equal keys in the sorted order.
-struct TokenSegments {
-    const int32_t *start, *stop;
-    const uint32_t* key;
-    int64_t rows;
-    __device__ __forceinline__ void bounds(int64_t v, int64_t& lo, int64_t& hi) const {
-        lo = start[v];
-        hi = stop[v];
-    }
-    __device__ __forceinline__ int64_t at(int64_t p) const {
-        const uint32_t k = key[p];
-        return k < rows ? (int64_t)k : -1;
-    }
+// A token's run of entries in the sorted order.
+struct Run {
+    int32_t token, lo, hi, reserved;
+};
+
+// A piece of a long segment: entries [lo, hi), piece `index` of `n`, the segment's first one at
+// `first` in the list.
+struct alignas(16) Piece {
+    int32_t segment, lo, hi, index, first, n, reserved[2];
+};
+// Long segments of one piece and the pieces of longer ones are listed apart: only those need
+// partial rows.  Rooms that ascending offsets stay within; what would pass them is dropped.
+struct PieceLists {
+    int32_t* count;              // of singles, of parts
+    Piece *singles, *parts;
+    int64_t most_singles, most_parts;
+    int32_t length;              // least entries of a piece
+    int32_t* arrived;            // [parts][piece tiles], used at a segment's first piece
+    float* partial;              // [parts][piece tiles * lanes * VE]
+    int32_t* partial_count;      // [parts][piece tiles]
 };
 
 struct SumArgs {
@@ -100,24 +126,38 @@ struct SumArgs {
     void* out;
     int64_t out_ld;
     int64_t n_segments, n_entries;
-    int dim, lanes_log2, tiles;  // lanes that share a row's tile, column tiles
-    int limit;                   // longest segment of one warp; pieces are this long
+    int dim, lanes_log2;         // lanes that share a row's tile
+    int tiles, piece_tiles;      // column tiles of a segment, and of a piece
     float scale;
     int mean;
     float* inv_counts;
-    float* partial;              // [chunks][2][tiles * lanes * VE]
-    int32_t* partial_count;      // [chunks][2]
+    // inner products with the segment's row of a second matrix
+    const void* dot_base;
+    int64_t dot_ld;
+    float* dot;                  // [tiles, or piece tiles of a long segment][n_entries], by position
+    PieceLists lists;
 };
 
+// VE elements in accesses of at most 16 bytes.
 template <class T, int VE>
-__device__ __forceinline__ void add_pack(float (&acc)[VE], const Pack<T, VE>& p, float c) {
+__device__ __forceinline__ Pack<T, VE> load_wide(const T* p) {
+    constexpr int N = VE * sizeof(T) > 16 ? 16 / sizeof(T) : VE;
+    Pack<T, VE> r;
 #pragma unroll
-    for (int e = 0; e < VE; ++e) acc[e] = fmaf(c, to_f32(p.v[e]), acc[e]);
+    for (int o = 0; o < VE; o += N) {
+        const Pack<T, N> q = load_pack<T, N>(p + o);
+#pragma unroll
+        for (int k = 0; k < N; ++k) r.v[o + k] = q.v[k];
+    }
+    return r;
 }
 
 // Stores VE results in accesses of at most 16 bytes.
 template <class TO, int VE>
-__device__ __forceinline__ void store_row(TO* p, const float (&acc)[VE], float factor) {
+__device__ __forceinline__ void store_row(TO* p, const float2 (&sum)[(VE + 1) / 2], float factor) {
+    float acc[VE];
+#pragma unroll
+    for (int k = 0; k < VE; ++k) acc[k] = k & 1 ? sum[k / 2].y : sum[k / 2].x;
     constexpr int N = VE * sizeof(TO) > 16 ? 16 / sizeof(TO) : VE;
 #pragma unroll
     for (int o = 0; o < VE; o += N) {
@@ -128,47 +168,14 @@ __device__ __forceinline__ void store_row(TO* p, const float (&acc)[VE], float f
     }
 }
 
-// The sum of entries [lo, hi) over this warp's column tile.  A row's tile is read by
-// 2^lanes_log2 lanes; the warp's 32 >> lanes_log2 lane groups take entries in turn and are
-// added at the end (every lane then holds the sum of its columns).  Returns the number of
-// counted entries.
-template <class T, int VE, class Entries>
-__device__ __forceinline__ int sum_entries(const Entries& entries, const SumArgs& a, int col, int64_t lo,
-                                           int64_t hi, float (&acc)[VE]) {
-    const int lane = threadIdx.x & 31, groups = 32 >> a.lanes_log2, group = lane >> a.lanes_log2;
-    const bool col_ok = col < a.dim;
-    const T* base = static_cast<const T*>(a.base) + col;
-    int count = 0;
-#pragma unroll
-    for (int e = 0; e < VE; ++e) acc[e] = 0.0f;
-    for (int64_t b = lo; b < hi; b += 32) {
-        const int n = (int)min((int64_t)32, hi - b);
-        int row = -1;
-        float coef = 0.0f;
-        if (lane < n) entries.get(b + lane, row, coef);
-        count += __popc(__ballot_sync(0xffffffffu, row >= 0));
-        for (int q = 0; q < n; q += kUnroll * groups) {
-            Pack<T, VE> p[kUnroll];
-            int r[kUnroll];
-            float c[kUnroll];
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-                const int i = q + u * groups + group;
-                r[u] = __shfl_sync(0xffffffffu, row, i & 31);
-                c[u] = __shfl_sync(0xffffffffu, coef, i & 31);
-                if (i >= n || !col_ok) r[u] = -1;
-                if (r[u] >= 0) p[u] = load_pack<T, VE>(base + (int64_t)r[u] * a.ld);
-            }
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
-                if (r[u] >= 0) add_pack<T, VE>(acc, p[u], c[u]);
-        }
-    }
-    for (int m = 16; m >= 1 << a.lanes_log2; m >>= 1)
-#pragma unroll
-        for (int e = 0; e < VE; ++e) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], m);
-    return count;
-}
+// The first column this lane works on (its vectors are 32 vectors apart), and the groups of lanes
+// that take entries in turn where a row is narrower than a warp.
+struct Lanes {
+    int lane, count, groups, group, col;
+    __device__ __forceinline__ Lanes(const SumArgs& a, int tile, int ve, int packs)
+        : lane(threadIdx.x & 31), count(1 << a.lanes_log2), groups(32 >> a.lanes_log2), group(lane >> a.lanes_log2),
+          col((((tile * packs) << a.lanes_log2) + (lane & (count - 1))) * ve) {}
+};
 
 // What a finished sum is multiplied by.
 __device__ __forceinline__ float finish_factor(const SumArgs& a, int64_t seg, int64_t count, bool write) {
@@ -180,101 +187,347 @@ __device__ __forceinline__ float finish_factor(const SumArgs& a, int64_t seg, in
     return a.scale * inv;
 }
 
-// One warp per (segment, column tile); segments longer than the limit are left to the
-// pieces.  Every other segment's row is written here, zeros for an empty one.
-template <class T, class TO, int VE, class Entries, class Segments>
-__global__ void __launch_bounds__(kThreads) segments_kernel(SumArgs a, Entries entries, Segments segs) {
-    const uint32_t w = blockIdx.x * kWarps + (threadIdx.x >> 5);
+// Sums of v[u] over each group's lanes, kDots at a time: 4 + 2 + 1 exchanges and one for each
+// remaining doubling.  The result is v[0], of the entry whose number is returned (the same in
+// lanes that differ below the group's width / kDots).
+__device__ __forceinline__ int reduce_dots(float (&v)[kDots], int lanes_log2, int lane) {
+    int entry = 0;
+#pragma unroll
+    for (int half = kDots / 2; half; half >>= 1) {
+        --lanes_log2;
+        const int bit = 1 << lanes_log2;
+        const bool up = lane & bit;
+#pragma unroll
+        for (int i = 0; i < half; ++i) {
+            const float keep = up ? v[i + half] : v[i], send = up ? v[i] : v[i + half];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, send, bit);
+        }
+        entry += up ? half : 0;
+    }
+    for (int bit = 1 << lanes_log2 >> 1; bit; bit >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], bit);
+    return entry;
+}
+
+// A warp's counted entries of a batch of 32.
+struct Batch {
+    int64_t at[32];  // byte offset of the row in the summed matrix
+    float coef[32];
+    int32_t pos[32];
+};
+
+template <int VE, int Packs>
+using Sums = float2[Packs][(VE + 1) / 2];
+
+// Entries q, q + groups, ... of a batch of n, N per group (all there when Full).  from[t]: vector
+// t of the matrix's first row; vectors behind the row's end are the last one's again.
+template <class T, int VE, int Packs, bool Dot, int N, bool Full>
+__device__ __forceinline__ void add_rows(const SumArgs& a, const Lanes& ln, const Batch& bt, const char* base, const int (&step)[Packs],
+                                         int q, int n, float2 (&acc)[Packs][(VE + 1) / 2], const float2 (&e)[Packs][(VE + 1) / 2],
+                                         float* dot) {
+    constexpr int H = (VE + 1) / 2;
+    Pack<T, VE> p[N][Packs];
+    float d[kDots] = {};
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+        const int i = q + u * ln.groups + ln.group;
+        if (Full || i < n) {
+            const T* row = reinterpret_cast<const T*>(base + bt.at[i]);
+#pragma unroll
+            for (int t = 0; t < Packs; ++t) p[u][t] = load_pack<T, VE>(row + step[t]);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+        const int i = q + u * ln.groups + ln.group;
+        if (!Full && i >= n) continue;
+        const float c = bt.coef[i];
+        float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int t = 0; t < Packs; ++t) {
+            float2 x[H];
+            unpack(p[u][t], x);
+#pragma unroll
+            for (int k = 0; k < H; ++k) {
+                acc[t][k] = fma2_rn(x[k], make_float2(c, c), acc[t][k]);
+                if (Dot) {
+                    if (ln.col + t * 32 * VE < a.dim) sum = fma2_rn(x[k], e[t][k], sum);
+                }
+            }
+        }
+        if (Dot) d[u] = sum.x + sum.y;
+    }
+    if constexpr (Dot) {
+        if (ln.count >= kDots) {
+            const int i = q + reduce_dots(d, a.lanes_log2, ln.lane) * ln.groups + ln.group;
+            if (i < n && i < q + N * ln.groups && (ln.lane & (ln.count / kDots - 1)) == 0) dot[bt.pos[i]] = d[0];
+        } else {
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                const int i = q + u * ln.groups + ln.group;
+                for (int bit = ln.count >> 1; bit; bit >>= 1) d[u] += __shfl_xor_sync(0xffffffffu, d[u], bit);
+                if (i < n && (ln.lane & (ln.count - 1)) == 0) dot[bt.pos[i]] = d[u];
+            }
+        }
+    }
+}
+
+// The sum of entries [lo, hi) over this warp's column tile, in every lane for its columns (vectors
+// behind the last column are another's and are not stored).  Returns the number of counted
+// entries.
+template <class T, class TE, int VE, int Packs, bool Dot, class Entries>
+__device__ __forceinline__ int sum_entries(const SumArgs& a, const Lanes& ln, Batch& bt, const Entries& entries, int64_t lo, int64_t hi,
+                                           const TE* dot_row, float* dot, float2 (&acc)[Packs][(VE + 1) / 2]) {
+    constexpr int H = (VE + 1) / 2, N = rows_ahead(Packs), Tail = (N + 1) / 2;
+    static_assert(N <= kDots, "reduce_dots takes a round's products");
+    int step[Packs];
+#pragma unroll
+    for (int t = 0; t < Packs; ++t) step[t] = ln.col + t * 32 * VE < a.dim ? ln.col + t * 32 * VE : 0;
+    const char* base = static_cast<const char*>(a.base);
+    float2 e[Packs][H];
+#pragma unroll
+    for (int t = 0; t < Packs; ++t)
+#pragma unroll
+        for (int k = 0; k < H; ++k) acc[t][k] = e[t][k] = make_float2(0.0f, 0.0f);
+    int row = -1, pos = 0, count = 0;
+    float coef = 0.0f;
+    auto look_up = [&](int64_t b) {
+        row = -1;
+        if (b + ln.lane < hi) {
+            entries.get(b + ln.lane, row, coef);
+            if (Dot) pos = entries.position(b + ln.lane);
+        }
+    };
+    look_up(lo);
+    if constexpr (Dot) {
+#pragma unroll
+        for (int t = 0; t < Packs; ++t) unpack(load_wide<TE, VE>(dot_row + step[t]), e[t]);
+    }
+    for (int64_t b = lo; b < hi; b += 32) {
+        const uint32_t counted = __ballot_sync(0xffffffffu, row >= 0);
+        const int n = __popc(counted);
+        __syncwarp();
+        if (row >= 0) {
+            const int i = __popc(counted & ((1u << ln.lane) - 1));
+            bt.at[i] = (int64_t)row * a.ld * (int)sizeof(T);
+            bt.coef[i] = coef;
+            if (Dot) bt.pos[i] = pos;
+        }
+        __syncwarp();
+        if (b + 32 < hi) look_up(b + 32);
+        count += n;
+        int q = 0;
+        for (; q + N * ln.groups <= n; q += N * ln.groups)
+            add_rows<T, VE, Packs, Dot, N, true>(a, ln, bt, base, step, q, n, acc, e, dot);
+        for (; q < n; q += Tail * ln.groups)
+            add_rows<T, VE, Packs, Dot, Tail, false>(a, ln, bt, base, step, q, n, acc, e, dot);
+    }
+    for (int m = 16; m >= ln.count; m >>= 1)
+#pragma unroll
+        for (int k = 0; k < H; ++k) {  // a narrow row has one vector a lane
+            acc[0][k].x += __shfl_xor_sync(0xffffffffu, acc[0][k].x, m);
+            acc[0][k].y += __shfl_xor_sync(0xffffffffu, acc[0][k].y, m);
+        }
+    return count;
+}
+
+// Stores a lane's vectors of a row.
+template <class TO, int VE, int Packs>
+__device__ __forceinline__ void store_sums(const SumArgs& a, const Lanes& ln, TO* row, const float2 (&acc)[Packs][(VE + 1) / 2],
+                                           float factor) {
+    if (ln.lane >= ln.count) return;
+#pragma unroll
+    for (int t = 0; t < Packs; ++t)
+        if (ln.col + t * 32 * VE < a.dim) store_row<TO, VE>(row + ln.col + t * 32 * VE, acc[t], factor);
+}
+
+// Lists a long segment's pieces (a whole warp's call).
+__device__ __forceinline__ void list_pieces(const SumArgs& a, int lane, int32_t seg, int32_t lo, int32_t hi) {
+    const PieceLists& l = a.lists;
+    // the square root: one after the other come a piece's entries and then the pieces
+    const int length = max(l.length, (int)sqrtf(1.5f * (float)(hi - lo)));
+    const int n = (hi - lo + length - 1) / length;
+    int32_t first = 0;
+    if (lane == 0) first = atomicAdd(l.count + (n > 1), n);
+    first = __shfl_sync(0xffffffffu, first, 0);
+    Piece* to = n > 1 ? l.parts : l.singles;
+    const int64_t room = n > 1 ? l.most_parts : l.most_singles;
+    if (first < 0) return;
+    for (int i = lane; i < n && first + (int64_t)i < room; i += 32)
+        to[first + (int64_t)i] = Piece{seg, lo + i * length, min(hi, lo + (i + 1) * length), i, first, n, {0, 0}};
+    if (n > 1 && first < room)
+        for (int t = lane; t < a.piece_tiles; t += 32) l.arrived[(int64_t)first * a.piece_tiles + t] = 0;
+}
+
+// A segment's row (of not more than kLimit entries) by one warp and column tile.
+template <class T, class TO, int VE, int Packs, bool Dot, class Entries>
+__device__ __forceinline__ void sum_segment(const SumArgs& a, const Lanes& ln, Batch& bt, const Entries& entries, int64_t seg, int64_t lo,
+                                            int64_t hi, int tile) {
+    float2 acc[Packs][(VE + 1) / 2];
+    const int count = sum_entries<T, TO, VE, Packs, Dot>(a, ln, bt, entries, lo, hi, static_cast<const TO*>(a.dot_base) + seg * a.dot_ld,
+                                                         a.dot + (int64_t)tile * a.n_entries, acc);
+    const float f = finish_factor(a, seg, count, tile == 0 && ln.lane == 0);
+    store_sums<TO, VE, Packs>(a, ln, static_cast<TO*>(a.out) + seg * a.out_ld, acc, f);
+}
+
+// Forward: one warp per (bag, column tile).
+template <class T, class TO, int VE, int Packs>
+__global__ void __launch_bounds__(kSegmentThreads, blocks_of_sm(Packs, VE, false)) bags_kernel(SumArgs a, TokenEntries entries, BagSegments bags) {
+    __shared__ Batch batch[kSegmentThreads / 32];
+    const uint32_t w = blockIdx.x * (kSegmentThreads / 32) + (threadIdx.x >> 5);
     const uint32_t seg = w / (uint32_t)a.tiles, tile = w - seg * (uint32_t)a.tiles;
     if (seg >= a.n_segments) return;
+    const Lanes ln(a, tile, VE, Packs);
     int64_t lo, hi;
-    segs.bounds(seg, lo, hi);
-    if (hi - lo > a.limit) return;
-    const int lane = threadIdx.x & 31, lanes = 1 << a.lanes_log2;
-    const int col = ((tile << a.lanes_log2) + (lane & (lanes - 1))) * VE;
-    float acc[VE];
-    const int count = sum_entries<T, VE>(entries, a, col, lo, hi, acc);
-    const float f = finish_factor(a, seg, count, tile == 0 && lane == 0);
-    if (lane < lanes && col < a.dim)
-        store_row<TO, VE>(static_cast<TO*>(a.out) + (int64_t)seg * a.out_ld + col, acc, f);
+    bags.bounds(seg, lo, hi);
+    if (hi - lo > kLimit) {
+        if (tile == 0) list_pieces(a, ln.lane, (int32_t)seg, (int32_t)lo, (int32_t)hi);
+        return;
+    }
+    sum_segment<T, TO, VE, Packs, false>(a, ln, batch[threadIdx.x >> 5], entries, seg, lo, hi, tile);
 }
 
-// One warp per (chunk of `limit` positions, column tile).  A segment longer than a chunk that
-// reaches into one holds its first position (slot 0) or its last (slot 1).
-template <class T, int VE, class Entries, class Segments>
-__global__ void __launch_bounds__(kThreads) pieces_kernel(SumArgs a, Entries entries, Segments segs) {
-    const uint32_t w = blockIdx.x * kWarps + (threadIdx.x >> 5);
-    const uint32_t chunk = w / (uint32_t)a.tiles, tile = w - chunk * (uint32_t)a.tiles;
-    const int64_t first = (int64_t)chunk * a.limit;
-    if (first >= a.n_entries) return;
-    const int64_t end = min(first + a.limit, a.n_entries);
-    const int lane = threadIdx.x & 31, lanes = 1 << a.lanes_log2;
-    const int col = ((tile << a.lanes_log2) + (lane & (lanes - 1))) * VE;
-    const int width = (a.tiles << a.lanes_log2) * VE;
-    const int64_t head = segs.at(first), tail = segs.at(end - 1);
-    for (int slot = 0; slot < 2; ++slot) {
-        const int64_t seg = slot ? tail : head;
-        if (seg < 0 || (slot && tail == head)) continue;
-        int64_t lo, hi;
-        segs.bounds(seg, lo, hi);
-        if (hi - lo <= a.limit) continue;
-        float acc[VE];
-        const int count = sum_entries<T, VE>(entries, a, col, max(lo, first), min(hi, end), acc);
-        if (lane < lanes) store_row<float, VE>(a.partial + ((int64_t)chunk * 2 + slot) * width + col, acc, 1.0f);
-        if (tile == 0 && lane == 0) a.partial_count[(int64_t)chunk * 2 + slot] = count;
+// Backward: one warp per (run, column tile), and behind those one per 32 table rows for the rows of
+// tokens without a run.
+template <class T, class TO, int VE, int Packs, bool Dot>
+__global__ void __launch_bounds__(kSegmentThreads, blocks_of_sm(Packs, VE, Dot))
+    runs_kernel(SumArgs a, SortedEntries entries, const Run* runs, const int32_t* n_runs, int64_t most_runs, const uint32_t* touched) {
+    __shared__ Batch batch[kSegmentThreads / 32];
+    const int64_t w = (int64_t)blockIdx.x * (kSegmentThreads / 32) + (threadIdx.x >> 5);
+    if (w < most_runs * a.tiles) {
+        const uint32_t r = (uint32_t)w / (uint32_t)a.tiles, tile = (uint32_t)w - r * (uint32_t)a.tiles;
+        if ((int)r >= *n_runs) return;
+        const Run run = runs[r];
+        const Lanes ln(a, tile, VE, Packs);
+        if (run.hi - run.lo > kLimit) {
+            if (tile == 0) list_pieces(a, ln.lane, run.token, run.lo, run.hi);
+            return;
+        }
+        sum_segment<T, TO, VE, Packs, Dot>(a, ln, batch[threadIdx.x >> 5], entries, run.token, run.lo, run.hi, tile);
+        return;
+    }
+    const int64_t first = (w - most_runs * a.tiles) * 32;
+    if (first >= a.n_segments) return;
+    const int64_t left = a.n_segments - first;
+    uint32_t rows = ~touched[first / 32];
+    if (left < 32) rows &= (1u << left) - 1;
+    const float2 zeros[Packs][(VE + 1) / 2] = {};
+    for (; rows; rows &= rows - 1)
+        for (int tile = 0; tile < a.tiles; ++tile)
+            store_sums<TO, VE, Packs>(a, Lanes(a, tile, VE, Packs),
+                                      static_cast<TO*>(a.out) + (first + __ffs(rows) - 1) * a.out_ld, zeros, 1.0f);
+}
+
+// One warp per (piece, column tile), one vector a lane: there may be few, and then a warp's time is
+// what counts.  The segment's last warp to arrive adds the pieces, in order.
+template <class T, class TO, int VE, bool Dot, class Entries>
+__global__ void __launch_bounds__(kSegmentThreads, Dot ? 12 : 14) pieces_kernel(SumArgs a, Entries entries) {
+    constexpr int Packs = 1;
+    __shared__ Batch batch[kSegmentThreads / 32];
+    const PieceLists& l = a.lists;
+    const int64_t n_parts = min((int64_t)max(l.count[1], 0), l.most_parts), n_singles = min((int64_t)max(l.count[0], 0), l.most_singles);
+    const int64_t items = (n_parts + n_singles) * a.piece_tiles;
+    const int width = (a.piece_tiles << a.lanes_log2) * VE;
+    constexpr int of_block = kSegmentThreads / 32;
+    for (int64_t item = (int64_t)blockIdx.x * of_block + (threadIdx.x >> 5); item < items; item += (int64_t)gridDim.x * of_block) {
+        const int64_t at = item / a.piece_tiles;
+        const int tile = (int)(item - at * a.piece_tiles);
+        const Lanes ln(a, tile, VE, Packs);
+        const Piece pc = at < n_parts ? l.parts[at] : l.singles[at - n_parts];
+        float2 acc[Packs][(VE + 1) / 2];
+        int count = sum_entries<T, TO, VE, Packs, Dot>(a, ln, batch[threadIdx.x >> 5], entries, pc.lo, pc.hi,
+                                                       static_cast<const TO*>(a.dot_base) + pc.segment * a.dot_ld,
+                                                       a.dot + (int64_t)tile * a.n_entries, acc);
+        if (pc.n > 1) {
+            if (ln.lane < ln.count) store_row<float, VE>(l.partial + at * width + ln.col, acc[0], 1.0f);
+            if (ln.lane == 0) l.partial_count[item] = count;
+            __threadfence();
+            __syncwarp();
+            int before = 0;
+            if (ln.lane == 0) before = atomicAdd(&l.arrived[(int64_t)pc.first * a.piece_tiles + tile], 1);
+            if (__shfl_sync(0xffffffffu, before, 0) != pc.n - 1) continue;
+            __threadfence();
+            count = 0;
+            const int n = (int)min((int64_t)pc.n, l.most_parts - pc.first);
+            if (a.mean) {
+                for (int i = ln.lane; i < n; i += 32) count += __ldcg(l.partial_count + (int64_t)(pc.first + i) * a.piece_tiles + tile);
+                count = __reduce_add_sync(0xffffffffu, count);
+            }
+#pragma unroll
+            for (int t = 0; t < Packs; ++t) {
+#pragma unroll
+                for (int k = 0; k < (VE + 1) / 2; ++k) acc[t][k] = make_float2(0.0f, 0.0f);
+                constexpr int kJoin = VE >= 4 ? 48 / VE : 16;  // partial rows on the way
+                for (int i0 = ln.group; i0 < n; i0 += kJoin * ln.groups) {
+                    float x[kJoin][VE];
+#pragma unroll
+                    for (int u = 0; u < kJoin; ++u) {
+                        const int i = i0 + u * ln.groups;
+                        const float* p = l.partial + (int64_t)(pc.first + min(i, n - 1)) * width + ln.col + t * 32 * VE;
+                        if constexpr (VE >= 4) {
+#pragma unroll
+                            for (int k = 0; k < VE; k += 4) {
+                                const float4 v = __ldcg(reinterpret_cast<const float4*>(p + k));
+                                x[u][k] = v.x, x[u][k + 1] = v.y, x[u][k + 2] = v.z, x[u][k + 3] = v.w;
+                            }
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < VE; ++k) x[u][k] = __ldcg(p + k);
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < kJoin; ++u)
+#pragma unroll
+                        for (int k = 0; k < VE; ++k)
+                            if (i0 + u * ln.groups < n) (k & 1 ? acc[t][k / 2].y : acc[t][k / 2].x) += x[u][k];
+                }
+                for (int m = 16; m >= ln.count; m >>= 1)
+#pragma unroll
+                    for (int k = 0; k < (VE + 1) / 2; ++k) {
+                        acc[t][k].x += __shfl_xor_sync(0xffffffffu, acc[t][k].x, m);
+                        acc[t][k].y += __shfl_xor_sync(0xffffffffu, acc[t][k].y, m);
+                    }
+            }
+        }
+        const float f = finish_factor(a, pc.segment, count, tile == 0 && ln.lane == 0);
+        store_sums<TO, VE, Packs>(a, ln, static_cast<TO*>(a.out) + (int64_t)pc.segment * a.out_ld, acc, f);
     }
 }
 
-// One block per (chunk, column tile): the long segment that starts in this chunk, if one
-// does, is the sum of its pieces.  The warps take pieces in turn and are added in order.
-template <class TO, int VE, class Segments>
-__global__ void __launch_bounds__(kThreads) join_kernel(SumArgs a, Segments segs) {
-    const uint32_t chunk = blockIdx.x / (uint32_t)a.tiles, tile = blockIdx.x - chunk * (uint32_t)a.tiles;
-    const int64_t first = (int64_t)chunk * a.limit, end = min(first + a.limit, a.n_entries);
-    const int64_t seg = segs.at(end - 1);
-    if (seg < 0) return;
-    int64_t lo, hi;
-    segs.bounds(seg, lo, hi);
-    if (hi - lo <= a.limit || lo < first || lo >= end) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lanes = 1 << a.lanes_log2;
-    const int groups = 32 >> a.lanes_log2, group = lane >> a.lanes_log2;
-    const int col = ((tile << a.lanes_log2) + (lane & (lanes - 1))) * VE;
-    const int width = (a.tiles << a.lanes_log2) * VE;
-    const int64_t last = (hi - 1) / a.limit, pieces = last - chunk + 1;
-    float acc[VE];
-    int64_t count = 0;
+// Bags of one token: a warp moves a column tile of kLookupRows rows.
+template <class T, class TO, int VE>
+__global__ void __launch_bounds__(kSegmentThreads) lookup_kernel(SumArgs a, TokenEntries entries) {
+    const uint32_t w = blockIdx.x * (kSegmentThreads / 32) + (threadIdx.x >> 5);
+    const uint32_t batch = w / (uint32_t)a.tiles, tile = w - batch * (uint32_t)a.tiles;
+    const Lanes ln(a, tile, VE, 1);
+    const int64_t first = (int64_t)batch * kLookupRows * ln.groups;
+    if (first >= a.n_segments) return;
+    const T* base = static_cast<const T*>(a.base) + ln.col;
+    Pack<T, VE> p[kLookupRows];
+    int row[kLookupRows];
+    float f[kLookupRows];
 #pragma unroll
-    for (int e = 0; e < VE; ++e) acc[e] = 0.0f;
-    for (int64_t p = warp * groups + group; p < pieces; p += kWarps * groups) {
-        const int64_t at = (chunk + p) * 2 + (p == 0 && lo > first ? 1 : 0);
-        count += a.partial_count[at];
-        const float* src = a.partial + at * width + col;
-#pragma unroll
-        for (int e = 0; e < VE; ++e) acc[e] += src[e];
+    for (int u = 0; u < kLookupRows; ++u) {
+        const int64_t i = first + u * ln.groups + ln.group;
+        row[u] = -1;
+        f[u] = 0.0f;
+        if (i < a.n_segments) entries.get(i, row[u], f[u]);
     }
-    for (int m = 16; m >= lanes; m >>= 1) {
-        count += __shfl_xor_sync(0xffffffffu, count, m);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], m);
+    for (int u = 0; u < kLookupRows; ++u)
+        if (row[u] >= 0 && ln.col < a.dim) p[u] = load_pack<T, VE>(base + (int64_t)row[u] * a.ld);
+#pragma unroll
+    for (int u = 0; u < kLookupRows; ++u) {
+        const int64_t i = first + u * ln.groups + ln.group;
+        if (i >= a.n_segments) continue;
+        float2 acc[(VE + 1) / 2] = {};
+        if (row[u] >= 0 && ln.col < a.dim) {
+            unpack(p[u], acc);
+#pragma unroll
+            for (int k = 0; k < (VE + 1) / 2; ++k) acc[k] = mul2_rn(acc[k], make_float2(f[u], f[u]));
+        }
+        if (a.mean && a.inv_counts && tile == 0 && (ln.lane & (ln.count - 1)) == 0) a.inv_counts[i] = 1.0f;
+        if (ln.col < a.dim) store_row<TO, VE>(static_cast<TO*>(a.out) + i * a.out_ld + ln.col, acc, a.scale);
     }
-    __shared__ float s_acc[kWarps][32 * VE];
-    __shared__ int64_t s_count[kWarps];
-#pragma unroll
-    for (int e = 0; e < VE; ++e) s_acc[warp][lane * VE + e] = acc[e];
-    if (lane == 0) s_count[warp] = count;
-    __syncthreads();
-    if (warp) return;
-    count = 0;
-#pragma unroll
-    for (int e = 0; e < VE; ++e) acc[e] = 0.0f;
-    for (int w = 0; w < kWarps; ++w) {
-        count += s_count[w];
-#pragma unroll
-        for (int e = 0; e < VE; ++e) acc[e] += s_acc[w][lane * VE + e];
-    }
-    const float f = finish_factor(a, seg, count, tile == 0 && lane == 0);
-    if (lane < lanes && col < a.dim)
-        store_row<TO, VE>(static_cast<TO*>(a.out) + seg * a.out_ld + col, acc, f);
 }
 
 // ---------------------------------------------------------------- sort by token
@@ -291,34 +544,107 @@ struct SortArgs {
     int32_t tiles;
     float scale;
     int shift, bins;
-    const uint32_t *key_in, *pos_in;
+    uint32_t *key_in, *pos_in;  // the first pass's count writes key_in, in position order
     uint32_t *key_out, *pos_out;
+    int32_t* bag;    // [n] by position, from the first pass
     int32_t* src;
     float* coef;
+    // zeroed by the first pass: bit maps of the tokens with a run, and with a long one; counts
+    uint32_t *touched, *lengthy;
+    int32_t *list_counts, *n_runs;
+    Run* runs;
+    int64_t most_runs;
     int32_t* hist;   // [bins][tiles]
     int32_t* total;  // [bins]
 };
 
-template <bool First>
-__device__ __forceinline__ uint32_t sort_key(const SortArgs& a, int64_t j) {
-    if (!First) return a.key_in[j];
-    const int64_t t = a.tokens[j];
-    if ((uint64_t)t >= (uint64_t)a.rows) return (uint32_t)a.rows;
-    if (a.bags.offsets && (j < a.bags.offsets[0] || j >= a.bags.offsets[a.bags.n_bags]))
-        return (uint32_t)a.rows;
-    return (uint32_t)t;
+// The bags of a tile's positions, into bag[]: the offset at or before the tile is searched for,
+// those inside it are marked at their positions (the last of equal ones counts), and the largest
+// mark up to a position is its bag.
+__device__ void tile_bags(const BagSegments& bags, int64_t base, int32_t (&bag)[kSortTile], int32_t* warp_max) {
+    if (!bags.offsets) {
+        for (int i = threadIdx.x; i < kSortTile; i += kThreads) bag[i] = (int32_t)(base + i);
+        __syncthreads();
+        return;
+    }
+    const int32_t before = (int32_t)bags.starts_up_to(base);
+    for (int i = threadIdx.x; i < kSortTile; i += kThreads) bag[i] = before;
+    __syncthreads();
+    for (int64_t k = before + threadIdx.x; k <= bags.n_bags; k += kThreads) {
+        const int64_t o = bags.offsets[k] - base;
+        if (o >= kSortTile) break;
+        if (o > 0) atomicMax(&bag[o], (int32_t)(k + 1));
+    }
+    __syncthreads();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int32_t v[kSortItems];
+#pragma unroll
+    for (int i = 0; i < kSortItems; ++i) {
+        v[i] = bag[threadIdx.x * kSortItems + i];
+        if (i) v[i] = max(v[i], v[i - 1]);
+    }
+    int32_t top = v[kSortItems - 1];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) top = max(top, __shfl_up_sync(0xffffffffu, top, d));
+    if (lane == 31) warp_max[warp] = top;
+    int32_t left = __shfl_up_sync(0xffffffffu, top, 1);
+    __syncthreads();
+    if (lane == 0) left = 0;
+    for (int w = 0; w < warp; ++w) left = max(left, warp_max[w]);
+#pragma unroll
+    for (int i = 0; i < kSortItems; ++i) {
+        const int32_t starts = max(v[i], left);  // offsets at or before the position
+        bag[threadIdx.x * kSortItems + i] = starts <= bags.n_bags ? starts - 1 : -1;
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ float entry_factor(const SortArgs& a, uint32_t pos, int32_t bag) {
+    float c = a.scale;
+    if (a.weights) c *= a.weights[pos];
+    if (a.inv_counts && bag >= 0) c *= a.inv_counts[bag];
+    return c;
+}
+__device__ __forceinline__ void clear_runs(const SortArgs& a) {  // every thread of the grid
+    const int64_t i0 = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i0 < 2) a.list_counts[i0] = 0;
+    if (i0 == 2) *a.n_runs = 0;
+    for (int64_t i = i0; i < (a.rows + 31) / 32; i += (int64_t)gridDim.x * blockDim.x) a.touched[i] = a.lengthy[i] = 0;
 }
 
 template <bool First>
 __global__ void __launch_bounds__(kThreads) sort_count_kernel(SortArgs a) {
     __shared__ int32_t count[kMaxBins];
+    __shared__ int32_t bag[First ? kSortTile : 1], warp_max[kWarps];
     for (int b = threadIdx.x; b < a.bins; b += kThreads) count[b] = 0;
-    __syncthreads();
     const int64_t base = (int64_t)blockIdx.x * kSortTile;
+    int64_t token[kSortItems];
+    if constexpr (First) {
+#pragma unroll
+        for (int i = 0; i < kSortItems; ++i) {
+            const int64_t j = base + i * kThreads + threadIdx.x;
+            token[i] = j < a.n ? a.tokens[j] : -1;
+        }
+        clear_runs(a);
+        tile_bags(a.bags, base, bag, warp_max);
+    } else {
+        __syncthreads();
+    }
 #pragma unroll
     for (int i = 0; i < kSortItems; ++i) {
-        const int64_t j = base + i * kThreads + threadIdx.x;
-        if (j < a.n) atomicAdd(&count[(sort_key<First>(a, j) >> a.shift) & (a.bins - 1)], 1);
+        const int at = i * kThreads + threadIdx.x;
+        const int64_t j = base + at;
+        if (j >= a.n) break;
+        uint32_t key;
+        if constexpr (First) {
+            // a position that counts nowhere has the key `rows` and no bag
+            const int32_t b = (uint64_t)token[i] < (uint64_t)a.rows ? bag[at] : -1;
+            key = b >= 0 ? (uint32_t)token[i] : (uint32_t)a.rows;
+            a.bag[j] = b;
+            a.key_in[j] = key;
+        } else {
+            key = a.key_in[j];
+        }
+        atomicAdd(&count[(key >> a.shift) & (a.bins - 1)], 1);
     }
     __syncthreads();
     for (int b = threadIdx.x; b < a.bins; b += kThreads) a.hist[(int64_t)b * a.tiles + blockIdx.x] = count[b];
@@ -359,7 +685,7 @@ __global__ void __launch_bounds__(kThreads) sort_move_kernel(SortArgs a) {
     for (int i = 0; i < kSortItems; ++i) {
         const int64_t j = base + i * 32 + lane;
         const bool in = j < a.n;
-        key[i] = in ? sort_key<First>(a, j) : 0;
+        key[i] = in ? a.key_in[j] : 0;
         const int d = (key[i] >> a.shift) & (a.bins - 1);
         const uint32_t peers = __match_any_sync(0xffffffffu, in ? d : -1);
         rank[i] = 0;
@@ -404,156 +730,208 @@ __global__ void __launch_bounds__(kThreads) sort_move_kernel(SortArgs a) {
         const int32_t to = seen[warp][(key[i] >> a.shift) & (a.bins - 1)] + rank[i];
         a.key_out[to] = key[i];
         const uint32_t pos = First ? (uint32_t)j : a.pos_in[j];
-        if (!Last) {
-            a.pos_out[to] = pos;
-            continue;
+        a.pos_out[to] = pos;
+        if (Last) {
+            const int32_t bag = a.bag[pos];
+            a.src[to] = bag;
+            a.coef[to] = entry_factor(a, pos, bag);
         }
-        const int64_t bag = key[i] < a.rows ? a.bags.at(pos) : -1;
-        float c = a.scale;
-        if (a.weights) c *= a.weights[pos];
-        if (a.inv_counts && bag >= 0) c *= a.inv_counts[bag];
-        a.src[to] = (int32_t)bag;
-        a.coef[to] = c;
     }
 }
 
-// Where each token's run begins and ends (both arrays start as zeros: tokens without a run).
-__global__ void __launch_bounds__(kThreads) sort_runs_kernel(const uint32_t* key, int32_t n, int64_t rows,
-                                                             int32_t* start, int32_t* stop) {
+// Lists each token's run; the thread at its first entry looks for its end, in steps that double.
+__global__ void __launch_bounds__(kThreads) sort_runs_kernel(SortArgs a, const uint32_t* key) {
     const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (i >= n) return;
-    const uint32_t k = key[i];
-    if (k >= rows) return;
-    if (i == 0 || key[i - 1] != k) start[k] = (int32_t)i;
-    if (i == n - 1 || key[i + 1] != k) stop[k] = (int32_t)(i + 1);
+    uint32_t k = (uint32_t)a.rows;
+    if (i < a.n) k = key[i];
+    const bool begins = k < a.rows && (i == 0 || key[i - 1] != k);
+    int64_t end = i + 1;
+    if (begins) {
+        int64_t in = i, step = 1;  // key[in] is k
+        while (in + step < a.n && key[in + step] == k) {
+            in += step;
+            step *= 2;
+        }
+        for (; step; step >>= 1)
+            if (in + step < a.n && key[in + step] == k) in += step;
+        end = in + 1;
+        atomicOr(a.touched + k / 32, 1u << (k & 31));
+        if (end - i > kLimit) atomicOr(a.lengthy + k / 32, 1u << (k & 31));
+    }
+    const int lane = threadIdx.x & 31;
+    const uint32_t who = __ballot_sync(0xffffffffu, begins);
+    int32_t at = 0;
+    if (lane == 0 && who) at = atomicAdd(a.n_runs, __popc(who));
+    at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1));
+    if (begins) a.runs[at] = Run{(int32_t)k, (int32_t)i, (int32_t)end, 0};
 }
 
-// ---------------------------------------------------------------- gradient of the weights
-// One warp per position: the inner product of its table row with its bag's gradient.
-template <class T, class TG>
-__global__ void __launch_bounds__(kThreads)
-    weights_grad_kernel(BagSegments bags, const int64_t* tokens, int64_t rows, const T* table, int64_t ld, int dim,
-                        const TG* grad, int64_t grad_ld, const float* inv_counts, float scale, float* d_weights) {
-    const int64_t j = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    if (j >= bags.n_tokens) return;
-    const int lane = threadIdx.x & 31;
-    const int64_t t = tokens[j];
-    const int64_t bag = (uint64_t)t < (uint64_t)rows ? bags.at(j) : -1;
-    float dot = 0.0f;
-    if (bag >= 0) {
-        const T* e = table + t * ld;
-        const TG* g = grad + bag * grad_ld;
-        for (int c = lane; c < dim; c += 32) dot = fmaf(to_f32(e[c]), to_f32(g[c]), dot);
+// dw_j: the column tiles' inner products in order, times scale / c_bag; 0 where j does not count.
+__global__ void __launch_bounds__(kThreads) weights_grad_kernel(const float* dot, int tiles, int piece_tiles, SortArgs a, float* d_weights) {
+    const int64_t j = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (j >= a.n) return;
+    const int32_t b = a.bag[j];
+    float v = 0.0f;
+    if (b >= 0) {
+        const uint32_t t = (uint32_t)a.tokens[j];
+        const int n = a.lengthy[t / 32] >> (t & 31) & 1 ? piece_tiles : tiles;
+        for (int i = 0; i < n; ++i) v += dot[(int64_t)i * a.n + j];
+        v *= a.inv_counts ? a.scale * a.inv_counts[b] : a.scale;
     }
-#pragma unroll
-    for (int m = 16; m; m >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, m);
-    if (lane == 0) {
-        float f = scale;
-        if (inv_counts && bag >= 0) f *= inv_counts[bag];
-        d_weights[j] = bag >= 0 ? dot * f : 0.0f;
-    }
+    d_weights[j] = v;
 }
 
 // ---------------------------------------------------------------- host
-struct Plan {
-    int lanes_log2, tiles, limit;
-    int64_t chunks;
-    int64_t width;  // floats of a partial row
+struct Matrix {
+    const void* p;
+    int64_t ld;
+    int size;  // of an element
 };
 
-// Widest access that every row of both matrices allows.
-int vector_elems(const void* in, int64_t in_ld, int in_size, const void* out, int64_t out_ld, int out_size, int dim) {
-    for (int ve = 16 / in_size; ve > 1; ve /= 2) {
-        if (in_size == 2 && ve == 2) break;  // 16-bit rows: 8, 4 or 1 elements
-        const int ib = ve * in_size, ob = std::min(16, ve * out_size);
-        if (dim % ve == 0 && (uintptr_t)in % ib == 0 && (in_ld * in_size) % ib == 0 && (uintptr_t)out % ob == 0 &&
-            (out_ld * out_size) % ob == 0)
-            return ve;
+// Elements per access that every row of the matrices allows: 16 bytes of the first one's, 8, 4, or
+// one element.
+int vector_elems(int dim, std::initializer_list<Matrix> all) {
+    for (int ve = 16 / all.begin()->size; ve > 1; ve /= 2) {
+        bool ok = dim % ve == 0;
+        for (const Matrix& m : all) {
+            const int bytes = std::min(16, ve * m.size);
+            ok = ok && (uintptr_t)m.p % bytes == 0 && (m.ld * m.size) % bytes == 0;
+        }
+        if (ok) return ve;
     }
     return 1;
 }
 
-Plan make_plan(int dim, int ve, int64_t n_entries) {
-    Plan p;
-    const int packs = (dim + ve - 1) / ve;
-    p.lanes_log2 = 0;
-    while (p.lanes_log2 < 5 && (1 << p.lanes_log2) < packs) ++p.lanes_log2;
-    p.tiles = (packs + (1 << p.lanes_log2) - 1) >> p.lanes_log2;
-    // at least 64 entries per piece, and at most about 4,096 pieces
-    p.limit = (int)std::max<int64_t>(64, (n_entries + 4095) / 4096);
-    p.chunks = (n_entries + p.limit - 1) / p.limit;
-    p.width = ((int64_t)p.tiles << p.lanes_log2) * ve;
-    return p;
-}
-
-// Bytes of the partial rows for any vector width (a row is padded to whole tiles).
 size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
-size_t partial_bytes(int64_t n_entries, int dim) {
-    const int64_t limit = std::max<int64_t>(64, (n_entries + 4095) / 4096);
-    if (n_entries <= limit) return 0;
-    const int64_t chunks = (n_entries + limit - 1) / limit;
-    const size_t width = (size_t)dim + 32 * 8;
-    return round256(chunks * 2 * width * sizeof(float)) + round256(chunks * 2 * sizeof(int32_t));
-}
 
+// Least entries of a long segment's pieces.
+int64_t piece_length(int64_t n_entries) { return std::max<int64_t>(kPiece, n_entries >> 14); }
+
+// Tiles of a row of dim elements: as many lanes as its vectors need, up to a warp, and then up to
+// `most` vectors a lane, as evenly as whole tiles allow.
+struct Tiling {
+    int lanes_log2 = 0, packs, tiles;
+    Tiling(int dim, int ve, int most) {
+        const int all = (dim + ve - 1) / ve;
+        while (lanes_log2 < 5 && (1 << lanes_log2) < all) ++lanes_log2;
+        tiles = (all + 32 * most - 1) / (32 * most);
+        packs = (all + 32 * tiles - 1) / (32 * tiles);
+    }
+};
+// Bounds for every vector width.
+int64_t most_tiles(int dim) { return (dim + 31) / 32; }
+int64_t most_width(int dim) { return (int64_t)dim + dim / 4 + 32 * 8 * 2; }
+
+// The workspace: taken piece by piece, or only counted (p null).
 struct Carver {
-    char* p;
+    char* p = nullptr;
     size_t used = 0;
     template <class T>
     T* take(size_t n) {
-        T* r = reinterpret_cast<T*>(p + used);
+        T* r = p ? reinterpret_cast<T*>(p + used) : nullptr;
         used += round256(n * sizeof(T));
         return r;
     }
 };
 
-template <class T, class TO, int VE, class Entries, class Segments>
-void launch_sum(SumArgs a, const Entries& entries, const Segments& segs, const Plan& p, cudaStream_t s) {
-    const int64_t warps = a.n_segments * p.tiles;
+// Lists and partial rows of long segments, for any tiling.
+void take_lists(SumArgs& a, Carver& ws) {
+    PieceLists& l = a.lists;
+    l.length = (int32_t)piece_length(a.n_entries);
+    l.most_singles = a.n_entries / kLimit;
+    l.most_parts = 2 * (a.n_entries / l.length);  // n > length entries have at most 2 n / length pieces
+    l.count = ws.take<int32_t>(2);
+    l.singles = ws.take<Piece>(l.most_singles);
+    l.parts = ws.take<Piece>(l.most_parts);
+    l.arrived = ws.take<int32_t>(l.most_parts * most_tiles(a.dim));
+    l.partial = ws.take<float>(l.most_parts * most_width(a.dim));
+    l.partial_count = ws.take<int32_t>(l.most_parts * most_tiles(a.dim));
+}
+
+unsigned grid_of(int64_t warps) {
     require(warps < (int64_t)1 << 32, "embed_bags: too many output tiles");
-    if (warps > 0) {
-        segments_kernel<T, TO, VE><<<(unsigned)((warps + kWarps - 1) / kWarps), kThreads, 0, s>>>(a, entries, segs);
+    constexpr int of_block = kSegmentThreads / 32;
+    return (unsigned)((warps + of_block - 1) / of_block);
+}
+
+// Launches the kernels of the sums; `b` and `so` are the forward and the backward call's.
+template <class T, class TO, int VE, bool Dot, class Entries>
+void launch_sum(SumArgs& a, const Entries& entries, const BagSegments& bags, const SortArgs& so, cudaStream_t s) {
+    constexpr bool forward = std::is_same_v<Entries, TokenEntries>, wide = VE * sizeof(T) == 16;
+    const Tiling narrow(a.dim, VE, 1), t(a.dim, VE, wide ? kMostPacks : 1);
+    a.lanes_log2 = t.lanes_log2;
+    a.tiles = t.tiles;
+    a.piece_tiles = narrow.tiles;
+    if (a.n_segments == 0) return;
+    if constexpr (forward) {
+        if (!bags.offsets) {
+            a.tiles = narrow.tiles;
+            const int64_t each = (int64_t)kLookupRows * (32 >> a.lanes_log2);
+            lookup_kernel<T, TO, VE><<<grid_of((a.n_segments + each - 1) / each * a.tiles), kSegmentThreads, 0, s>>>(a, entries);
+            HANNS_CUDA_OK(cudaGetLastError());
+            return;
+        }
+    }
+    auto launch = [&](auto packs) {
+        constexpr int Packs = decltype(packs)::value;
+        if constexpr (forward) {
+            bags_kernel<T, TO, VE, Packs><<<grid_of(a.n_segments * a.tiles), kSegmentThreads, 0, s>>>(a, entries, bags);
+        } else {
+            const int64_t warps = so.most_runs * a.tiles + (a.n_segments + 31) / 32;
+            runs_kernel<T, TO, VE, Packs, Dot><<<grid_of(warps), kSegmentThreads, 0, s>>>(a, entries, so.runs, so.n_runs, so.most_runs,
+                                                                                          so.touched);
+        }
         HANNS_CUDA_OK(cudaGetLastError());
+    };
+    if constexpr (wide) {
+        switch (t.packs) {
+            case 1: launch(std::integral_constant<int, 1>()); break;
+            case 2: launch(std::integral_constant<int, 2>()); break;
+            case 3: launch(std::integral_constant<int, 3>()); break;
+            default: launch(std::integral_constant<int, 4>());
+        }
+    } else {
+        launch(std::integral_constant<int, 1>());
     }
-    if (a.n_entries <= p.limit || warps == 0) return;
-    const int64_t pw = p.chunks * p.tiles;
-    pieces_kernel<T, VE><<<(unsigned)((pw + kWarps - 1) / kWarps), kThreads, 0, s>>>(a, entries, segs);
-    HANNS_CUDA_OK(cudaGetLastError());
-    join_kernel<TO, VE><<<(unsigned)pw, kThreads, 0, s>>>(a, segs);
+    if (a.n_entries <= kLimit) return;
+    const int64_t most = (a.lists.most_singles + a.lists.most_parts) * a.piece_tiles;
+    pieces_kernel<T, TO, VE, Dot><<<(unsigned)std::min<int64_t>(grid_of(most), 16 * 148), kSegmentThreads, 0, s>>>(a, entries);
     HANNS_CUDA_OK(cudaGetLastError());
 }
 
-template <class T, class TO, class Entries, class Segments>
-void sum_segments(SumArgs a, const Entries& entries, const Segments& segs, Carver& ws, cudaStream_t s) {
-    const int ve = vector_elems(a.base, a.ld, sizeof(T), a.out, a.out_ld, sizeof(TO), a.dim);
-    const Plan p = make_plan(a.dim, ve, a.n_entries);
-    a.lanes_log2 = p.lanes_log2;
-    a.tiles = p.tiles;
-    a.limit = p.limit;
-    if (a.n_entries > p.limit) {
-        a.partial = ws.take<float>(p.chunks * 2 * p.width);
-        a.partial_count = ws.take<int32_t>(p.chunks * 2);
-    }
+// In: type of the summed rows, Out: of the result (and of the rows of the inner products).
+template <class T, class TO, bool Dot, class Entries>
+void sum_segments(SumArgs& a, const Entries& entries, const BagSegments& bags, const SortArgs& so, cudaStream_t s) {
+    const Matrix in{a.base, a.ld, sizeof(T)}, out{a.out, a.out_ld, sizeof(TO)};
+    const int ve = Dot ? vector_elems(a.dim, {in, out, Matrix{a.dot_base, a.dot_ld, sizeof(TO)}}) : vector_elems(a.dim, {in, out});
     constexpr int wide = 16 / sizeof(T);
-    if (ve == wide) launch_sum<T, TO, wide>(a, entries, segs, p, s);
-    else if (ve == wide / 2) launch_sum<T, TO, wide / 2>(a, entries, segs, p, s);
-    else launch_sum<T, TO, 1>(a, entries, segs, p, s);
+    if (ve == wide) return launch_sum<T, TO, wide, Dot>(a, entries, bags, so, s);
+    if (ve == wide / 2) return launch_sum<T, TO, wide / 2, Dot>(a, entries, bags, so, s);
+    if constexpr (wide == 8) {
+        if (ve == 2) return launch_sum<T, TO, 2, Dot>(a, entries, bags, so, s);
+    }
+    launch_sum<T, TO, 1, Dot>(a, entries, bags, so, s);
 }
 
-template <class Entries, class Segments>
-void sum_typed(int32_t in, int32_t out, const SumArgs& a, const Entries& e, const Segments& g, Carver& ws,
-               cudaStream_t s) {
-    if (in == HANNS_DTYPE_F32) {
-        if (out == HANNS_DTYPE_F32) return sum_segments<float, float>(a, e, g, ws, s);
-        if (out == HANNS_DTYPE_F16) return sum_segments<float, __half>(a, e, g, ws, s);
-        return sum_segments<float, __nv_bfloat16>(a, e, g, ws, s);
-    }
+// Forward: from a table's type to the same or f32; backward the other way.
+void sum_bags(int32_t in, int32_t out, SumArgs& a, const TokenEntries& e, const BagSegments& bags, cudaStream_t s) {
+    const SortArgs none{};
+    if (in == HANNS_DTYPE_F32) return sum_segments<float, float, false>(a, e, bags, none, s);
     if (in == HANNS_DTYPE_F16) {
-        if (out == HANNS_DTYPE_F32) return sum_segments<__half, float>(a, e, g, ws, s);
-        return sum_segments<__half, __half>(a, e, g, ws, s);
+        if (out == HANNS_DTYPE_F32) return sum_segments<__half, float, false>(a, e, bags, none, s);
+        return sum_segments<__half, __half, false>(a, e, bags, none, s);
     }
-    if (out == HANNS_DTYPE_F32) return sum_segments<__nv_bfloat16, float>(a, e, g, ws, s);
-    return sum_segments<__nv_bfloat16, __nv_bfloat16>(a, e, g, ws, s);
+    if (out == HANNS_DTYPE_F32) return sum_segments<__nv_bfloat16, float, false>(a, e, bags, none, s);
+    sum_segments<__nv_bfloat16, __nv_bfloat16, false>(a, e, bags, none, s);
+}
+template <bool Dot>
+void sum_runs(int32_t in, int32_t out, SumArgs& a, const SortedEntries& e, const SortArgs& so, cudaStream_t s) {
+    const BagSegments none{};
+    if (in == HANNS_DTYPE_F16) return sum_segments<__half, __half, Dot>(a, e, none, so, s);
+    if (in == HANNS_DTYPE_BF16) return sum_segments<__nv_bfloat16, __nv_bfloat16, Dot>(a, e, none, so, s);
+    if (out == HANNS_DTYPE_F32) return sum_segments<float, float, Dot>(a, e, none, so, s);
+    if (out == HANNS_DTYPE_F16) return sum_segments<float, __half, Dot>(a, e, none, so, s);
+    sum_segments<float, __nv_bfloat16, Dot>(a, e, none, so, s);
 }
 
 void check_bags(const hanns_embed_bags_t* b) {
@@ -587,15 +965,6 @@ SortPlan sort_plan(int64_t rows, int64_t n) {
     return p;
 }
 
-size_t grad_bytes(const hanns_embed_bags_t* b) {
-    if (b->n_tokens == 0) return round256(b->rows * sizeof(int32_t)) * 2;
-    const SortPlan sp = sort_plan(b->rows, b->n_tokens);
-    size_t t = 6 * round256(b->n_tokens * 4);
-    t += round256(((size_t)sp.tiles << sp.bits) * 4) + round256(((size_t)1 << sp.bits) * 4);
-    t += 2 * round256(b->rows * sizeof(int32_t));
-    return t + partial_bytes(b->n_tokens, b->dim);
-}
-
 template <bool First>
 void sort_pass(const SortArgs& a, bool last, cudaStream_t s) {
     sort_count_kernel<First><<<a.tiles, kThreads, 0, s>>>(a);
@@ -605,14 +974,32 @@ void sort_pass(const SortArgs& a, bool last, cudaStream_t s) {
     HANNS_CUDA_OK(cudaGetLastError());
 }
 
-template <class T, class TG>
-void launch_weights_grad(const hanns_embed_bags_t* b, const BagSegments& bags, const void* grad, int64_t grad_ld,
-                         float* d_weights, cudaStream_t s) {
-    weights_grad_kernel<T, TG><<<(unsigned)((b->n_tokens + kWarps - 1) / kWarps), kThreads, 0, s>>>(
-        bags, b->tokens, b->rows, static_cast<const T*>(b->table), b->ld, b->dim, static_cast<const TG*>(grad), grad_ld,
-        b->mean ? b->inv_counts : nullptr, b->scale, d_weights);
-    HANNS_CUDA_OK(cudaGetLastError());
-}
+// Workspace of a gradient call, carved alike when it is counted and when it is used.
+struct GradSpace {
+    SumArgs sum{};
+    SortArgs sort{};
+    uint32_t* key[2];
+    uint32_t* pos[2];
+    GradSpace(const hanns_embed_bags_t* b, const SortPlan& sp, Carver& ws) {
+        const size_t n = (size_t)b->n_tokens;
+        sort.touched = ws.take<uint32_t>((b->rows + 31) / 32);
+        sort.lengthy = ws.take<uint32_t>((b->rows + 31) / 32);
+        sort.n_runs = ws.take<int32_t>(1);
+        sort.most_runs = std::min<int64_t>(b->rows, b->n_tokens);
+        sort.runs = ws.take<Run>(sort.most_runs);
+        for (auto* k : {&key[0], &key[1], &pos[0], &pos[1]}) *k = ws.take<uint32_t>(n);
+        sort.bag = ws.take<int32_t>(n);
+        sort.src = ws.take<int32_t>(n);
+        sort.coef = ws.take<float>(n);
+        sort.hist = ws.take<int32_t>((size_t)sp.tiles << sp.bits);
+        sort.total = ws.take<int32_t>((size_t)1 << sp.bits);
+        sum.dim = b->dim;
+        sum.n_entries = b->n_tokens;
+        take_lists(sum, ws);
+        sort.list_counts = sum.lists.count;
+        sum.dot = ws.take<float>(b->weights ? n * most_tiles(b->dim) : 0);
+    }
+};
 
 }  // namespace
 }  // namespace hanns
@@ -621,8 +1008,16 @@ void launch_weights_grad(const hanns_embed_bags_t* b, const BagSegments& bags, c
 extern "C" int64_t hanns_gpu_embed_bags_workspace_bytes(const hanns_embed_bags_t* b) {
     int64_t n = -1;
     hanns::operator_entry([&] {
-        hanns::check_bags(b);
-        n = (int64_t)hanns::partial_bytes(b->n_tokens, b->dim);
+        using namespace hanns;
+        check_bags(b);
+        n = 0;
+        if (!b->offsets || b->n_tokens <= kLimit) return;  // no bag can be long
+        Carver ws;
+        SumArgs a{};
+        a.dim = b->dim;
+        a.n_entries = b->n_tokens;
+        take_lists(a, ws);
+        n = (int64_t)ws.used;
     });
     return n;
 }
@@ -633,8 +1028,8 @@ extern "C" int32_t hanns_gpu_embed_bags_device(const hanns_embed_bags_t* b, void
         check_bags(b);
         if (b->n_bags == 0) return;
         require(b->table && b->out && (b->tokens || b->n_tokens == 0), "embed_bags: null table, tokens or out");
-        check_workspace(partial_bytes(b->n_tokens, b->dim), b->workspace, b->workspace_bytes);
-        Carver ws{static_cast<char*>(b->workspace)};
+        check_workspace((size_t)hanns_gpu_embed_bags_workspace_bytes(b), b->workspace, b->workspace_bytes);
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
         SumArgs a{};
         a.base = b->table;
         a.ld = b->ld;
@@ -646,16 +1041,24 @@ extern "C" int32_t hanns_gpu_embed_bags_device(const hanns_embed_bags_t* b, void
         a.scale = b->scale;
         a.mean = b->mean != 0;
         a.inv_counts = b->inv_counts;
-        sum_typed(b->dtype, b->out_dtype, a, TokenEntries{b->tokens, b->weights, b->rows},
-                  BagSegments{b->offsets, b->n_bags, b->n_tokens}, ws, static_cast<cudaStream_t>(stream));
+        if (b->offsets && b->n_tokens > kLimit) {
+            Carver ws{static_cast<char*>(b->workspace)};
+            take_lists(a, ws);
+            HANNS_CUDA_OK(cudaMemsetAsync(a.lists.count, 0, 2 * sizeof(int32_t), s));
+        }
+        sum_bags(b->dtype, b->out_dtype, a, TokenEntries{b->tokens, b->weights, b->rows},
+                 BagSegments{b->offsets, b->n_bags, b->n_tokens}, s);
     });
 }
 
 extern "C" int64_t hanns_gpu_embed_bags_grad_workspace_bytes(const hanns_embed_bags_t* b) {
     int64_t n = -1;
     hanns::operator_entry([&] {
-        hanns::check_bags(b);
-        n = (int64_t)hanns::grad_bytes(b);
+        using namespace hanns;
+        check_bags(b);
+        Carver ws;
+        GradSpace(b, sort_plan(b->rows, b->n_tokens), ws);
+        n = (int64_t)ws.used;
     });
     return n;
 }
@@ -666,78 +1069,61 @@ extern "C" int32_t hanns_gpu_embed_bags_grad_device(const hanns_embed_bags_t* b,
     return hanns::operator_entry([&] {
         using namespace hanns;
         check_bags(b);
+        if (!d_table && !d_weights) return;
+        require(d_table, "embed_bags: the weights' gradient comes with the table's");
         require(grad || b->n_bags == 0, "embed_bags: null gradient");
         require(b->tokens || b->n_tokens == 0, "embed_bags: null tokens");
         require(!b->mean || b->inv_counts || b->n_bags == 0, "embed_bags: a mean's gradient needs inv_counts");
+        require(!d_weights || (b->table && b->weights), "embed_bags: the weights' gradient needs the table and the weights");
+        check_workspace((size_t)hanns_gpu_embed_bags_grad_workspace_bytes(b), b->workspace, b->workspace_bytes);
         cudaStream_t s = static_cast<cudaStream_t>(stream);
-        const BagSegments bags{b->offsets, b->n_bags, b->n_tokens};
-        if (d_weights && b->n_tokens > 0) {
-            require(b->table, "embed_bags: the weights' gradient needs the table");
-            const bool g32 = b->out_dtype == HANNS_DTYPE_F32;
-            if (b->dtype == HANNS_DTYPE_F32) launch_weights_grad<float, float>(b, bags, grad, grad_ld, d_weights, s);
-            else if (b->dtype == HANNS_DTYPE_F16) {
-                if (g32) launch_weights_grad<__half, float>(b, bags, grad, grad_ld, d_weights, s);
-                else launch_weights_grad<__half, __half>(b, bags, grad, grad_ld, d_weights, s);
-            } else {
-                if (g32) launch_weights_grad<__nv_bfloat16, float>(b, bags, grad, grad_ld, d_weights, s);
-                else launch_weights_grad<__nv_bfloat16, __nv_bfloat16>(b, bags, grad, grad_ld, d_weights, s);
-            }
-        }
-        if (!d_table) return;
-        check_workspace(grad_bytes(b), b->workspace, b->workspace_bytes);
+        const SortPlan sp = sort_plan(b->rows, b->n_tokens);
         Carver ws{static_cast<char*>(b->workspace)};
-        int32_t* start = ws.take<int32_t>(b->rows);
-        int32_t* stop = ws.take<int32_t>(b->rows);
-        HANNS_CUDA_OK(cudaMemsetAsync(start, 0, (char*)stop - (char*)start + b->rows * sizeof(int32_t), s));
-        const size_t n = (size_t)b->n_tokens;
-        uint32_t* key[2] = {nullptr, nullptr};
-        uint32_t* pos[2] = {nullptr, nullptr};
-        int32_t* src = nullptr;
-        float* coef = nullptr;
-        uint32_t* sorted = nullptr;
-        if (n > 0) {
-            const SortPlan sp = sort_plan(b->rows, b->n_tokens);
-            for (auto* k : {&key[0], &key[1], &pos[0], &pos[1]}) *k = ws.take<uint32_t>(n);
-            src = ws.take<int32_t>(n);
-            coef = ws.take<float>(n);
-            SortArgs a{};
-            a.bags = bags;
-            a.tokens = b->tokens;
-            a.weights = b->weights;
-            a.inv_counts = b->mean ? b->inv_counts : nullptr;
-            a.rows = b->rows;
-            a.n = (int32_t)n;
-            a.tiles = sp.tiles;
-            a.scale = b->scale;
-            a.bins = 1 << sp.bits;
-            a.src = src;
-            a.coef = coef;
-            a.hist = ws.take<int32_t>((size_t)sp.tiles << sp.bits);
-            a.total = ws.take<int32_t>((size_t)1 << sp.bits);
+        GradSpace gs(b, sp, ws);
+        SortArgs& so = gs.sort;
+        const int32_t n = (int32_t)b->n_tokens;
+        so.bags = BagSegments{b->offsets, b->n_bags, b->n_tokens};
+        so.tokens = b->tokens;
+        so.weights = b->weights;
+        so.inv_counts = b->mean ? b->inv_counts : nullptr;
+        so.rows = b->rows;
+        so.n = n;
+        so.tiles = sp.tiles;
+        so.scale = b->scale;
+        so.bins = 1 << sp.bits;
+        const uint32_t *sorted = nullptr, *position = nullptr;
+        if (n == 0) {
+            HANNS_CUDA_OK(cudaMemsetAsync(so.touched, 0, (b->rows + 31) / 32 * sizeof(uint32_t), s));
+            HANNS_CUDA_OK(cudaMemsetAsync(so.n_runs, 0, sizeof(int32_t), s));
+        } else {
             for (int p = 0; p < sp.passes; ++p) {
-                a.shift = p * sp.bits;
-                a.key_in = key[(p + 1) & 1];
-                a.pos_in = pos[(p + 1) & 1];
-                a.key_out = key[p & 1];
-                a.pos_out = pos[p & 1];
-                if (p == 0) sort_pass<true>(a, sp.passes == 1, s);
-                else sort_pass<false>(a, p == sp.passes - 1, s);
+                so.shift = p * sp.bits;
+                so.key_in = gs.key[p & 1];
+                so.pos_in = gs.pos[p & 1];
+                so.key_out = gs.key[(p + 1) & 1];
+                so.pos_out = gs.pos[(p + 1) & 1];
+                if (p == 0) sort_pass<true>(so, sp.passes == 1, s);
+                else sort_pass<false>(so, p == sp.passes - 1, s);
             }
-            sorted = key[(sp.passes - 1) & 1];
-            sort_runs_kernel<<<(unsigned)((n + kThreads - 1) / kThreads), kThreads, 0, s>>>(sorted, (int32_t)n, b->rows,
-                                                                                           start, stop);
+            sorted = gs.key[sp.passes & 1];
+            position = gs.pos[sp.passes & 1];
+            sort_runs_kernel<<<(unsigned)(((int64_t)n + kThreads - 1) / kThreads), kThreads, 0, s>>>(so, sorted);
             HANNS_CUDA_OK(cudaGetLastError());
         }
-        SumArgs a{};
+        SumArgs& a = gs.sum;
         a.base = grad;
         a.ld = grad_ld;
         a.out = d_table;
         a.out_ld = d_table_ld;
         a.n_segments = b->rows;
-        a.n_entries = b->n_tokens;
-        a.dim = b->dim;
         a.scale = 1.0f;
-        sum_typed(b->out_dtype, b->dtype, a, SortedEntries{src, coef}, TokenSegments{start, stop, sorted, b->rows}, ws,
-                  s);
+        const SortedEntries entries{so.src, so.coef, position};
+        if (!d_weights || n == 0) return sum_runs<false>(b->out_dtype, b->dtype, a, entries, so, s);
+        a.dot_base = b->table;
+        a.dot_ld = b->ld;
+        sum_runs<true>(b->out_dtype, b->dtype, a, entries, so, s);
+        weights_grad_kernel<<<(unsigned)(((int64_t)n + kThreads - 1) / kThreads), kThreads, 0, s>>>(a.dot, a.tiles, a.piece_tiles, so,
+                                                                                                   d_weights);
+        HANNS_CUDA_OK(cudaGetLastError());
     });
 }

@@ -68,4 +68,28 @@ __device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
     return *reinterpret_cast<const Pack<T, N>*>(p);
 }
 
+// Two 16-bit elements in a word, as f32.
+template <class T> __device__ __forceinline__ float2 pair_f32(uint32_t w);
+template <> __device__ __forceinline__ float2 pair_f32<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <> __device__ __forceinline__ float2 pair_f32<__half>(uint32_t w) {
+    return __half22float2(*reinterpret_cast<__half2*>(&w));
+}
+
+// A pack's elements as f32 pairs (one element: in the first lane).
+template <class T, int N>
+__device__ __forceinline__ void unpack(const Pack<T, N>& p, float2 (&x)[(N + 1) / 2]) {
+    if constexpr (N == 1) {
+        x[0] = make_float2(to_f32(p.v[0]), 0.0f);
+    } else if constexpr (sizeof(T) == 2) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&p);
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) x[i] = pair_f32<T>(w[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) x[i] = make_float2(to_f32(p.v[2 * i]), to_f32(p.v[2 * i + 1]));
+    }
+}
+
 }  // namespace hanns

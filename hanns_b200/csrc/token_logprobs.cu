@@ -116,15 +116,8 @@ struct RowView {
     __device__ __forceinline__ int vectors() const { return (int)(((int64_t)lead + vocab + VE - 1) / VE); }
 };
 
-// Two 16-bit elements in a word: their f32, and the larger of two words' elements (`max_pairs`
-// keeps a NaN, `raise_pairs` drops it).
-template <class T> __device__ __forceinline__ float2 pair_f32(uint32_t w);
-template <> __device__ __forceinline__ float2 pair_f32<__nv_bfloat16>(uint32_t w) {
-    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-template <> __device__ __forceinline__ float2 pair_f32<__half>(uint32_t w) {
-    return __half22float2(*reinterpret_cast<__half2*>(&w));
-}
+// The larger of two words' 16-bit elements, two by two (`max_pairs` keeps a NaN, `raise_pairs`
+// drops it).
 template <class T> __device__ __forceinline__ uint32_t max_pairs(uint32_t a, uint32_t b);
 template <> __device__ __forceinline__ uint32_t max_pairs<__nv_bfloat16>(uint32_t a, uint32_t b) {
     uint32_t r;

@@ -128,23 +128,19 @@ def _embed_bags_grad(grad, table, tokens, offsets, weights, inv, scale, mean, ou
                      want_weights):
     dev = table.device
     grad = _rows(grad)
-    d_table = d_weights = None
-    if want_table:
-        d_table = torch.empty(table.shape, dtype=table.dtype, device=dev)
-    if want_weights:
-        d_weights = torch.empty(tokens.numel(), dtype=torch.float32, device=dev)
+    # the weights' gradient is a by-product of the table's
+    d_table = torch.empty(table.shape, dtype=table.dtype, device=dev)
+    d_weights = torch.empty(tokens.shape[0], dtype=torch.float32, device=dev) if want_weights else None
     b = _bags(table, tokens, offsets, weights, scale, mean, out_dtype, inv)
     lib, ref = L.lib(), C.byref(b)
 
     def work(stream):
-        ws = None  # noqa: F841 (kept until enqueued)
-        if want_table:
-            ws = _workspace(lib.hanns_gpu_embed_bags_grad_workspace_bytes(ref), dev, b)  # noqa: F841
-        _check(lib.hanns_gpu_embed_bags_grad_device(ref, grad.data_ptr(), grad.stride(0), _ptr(d_table), table.shape[1],
-                                                    _ptr(d_weights), stream), "embed_bags")
+        ws = _workspace(lib.hanns_gpu_embed_bags_grad_workspace_bytes(ref), dev, b)  # noqa: F841 (kept until enqueued)
+        _check(lib.hanns_gpu_embed_bags_grad_device(ref, grad.data_ptr(), grad.stride(0), d_table.data_ptr(),
+                                                    table.shape[1], _ptr(d_weights), stream), "embed_bags")
 
     _run(dev, work)
-    return d_table, d_weights
+    return d_table if want_table else None, d_weights
 
 
 def embed_bags(table, tokens, offsets=None, weights=None, *, scale: float = 1.0, mean: bool = False,

@@ -410,11 +410,11 @@ typedef struct {
 } hanns_embed_bags_t;
 int64_t hanns_gpu_embed_bags_workspace_bytes(const hanns_embed_bags_t* bags);
 int32_t hanns_gpu_embed_bags_device(const hanns_embed_bags_t* bags, void* stream);
-/* Gradients from grad (n_bags rows of dim, out_dtype, grad_ld elements apart): d_table (may be
- * NULL; rows x dim of the table's type, every row written) and d_weights (may be NULL;
- * n_tokens, zero for positions that do not count).  A token's terms are added in the order
- * of its positions: results do not change from run to run.  `out` is not read; a mean needs
- * the forward call's inv_counts; table may be NULL when d_weights is. */
+/* Gradients from grad (n_bags rows of dim, out_dtype, grad_ld elements apart): d_table (rows x
+ * dim of the table's type, every row written) and, where there are weights, d_weights (may be
+ * NULL; n_tokens, zero for positions that do not count).  A token's terms are added in the
+ * order of its positions: results do not change from run to run.  `out` is not read; a mean
+ * needs the forward call's inv_counts; table may be NULL when d_weights is. */
 int64_t hanns_gpu_embed_bags_grad_workspace_bytes(const hanns_embed_bags_t* bags);
 int32_t hanns_gpu_embed_bags_grad_device(const hanns_embed_bags_t* bags, const void* grad,
                                          int64_t grad_ld, void* d_table, int64_t d_table_ld,
