@@ -40,7 +40,7 @@ constexpr int kDots = 8;              // inner products that are reduced togethe
 // that its registers are kept to (more spill, fewer leave the memory idle).
 constexpr int kMostPacks = 4;
 __host__ __device__ constexpr int rows_ahead(int packs) { return packs == 1 ? 8 : packs == 2 ? 3 : 2; }
-constexpr int blocks_of_sm(int packs, int ve, bool dot) { return packs == 1 ? 14 : ve == 8 ? (dot ? 10 : 16) : dot ? 14 : 18; }
+constexpr int blocks_of_sm(int packs, int ve, bool forward) { return packs == 1 ? 14 : forward ? (ve == 8 ? 16 : 18) : ve == 8 ? 10 : 14; }
 constexpr int kLookupRows = 8;        // rows of a warp in a lookup
 constexpr int kMaxBinBits = 9, kMaxBins = 1 << kMaxBinBits;
 constexpr int kSortItems = 4, kSortTile = kThreads * kSortItems;
@@ -371,7 +371,7 @@ __device__ __forceinline__ void sum_segment(const SumArgs& a, const Lanes& ln, B
 
 // Forward: one warp per (bag, column tile).
 template <class T, class TO, int VE, int Packs>
-__global__ void __launch_bounds__(kSegmentThreads, blocks_of_sm(Packs, VE, false)) bags_kernel(SumArgs a, TokenEntries entries, BagSegments bags) {
+__global__ void __launch_bounds__(kSegmentThreads, blocks_of_sm(Packs, VE, true)) bags_kernel(SumArgs a, TokenEntries entries, BagSegments bags) {
     __shared__ Batch batch[kSegmentThreads / 32];
     const uint32_t w = blockIdx.x * (kSegmentThreads / 32) + (threadIdx.x >> 5);
     const uint32_t seg = w / (uint32_t)a.tiles, tile = w - seg * (uint32_t)a.tiles;
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(kSegmentThreads, blocks_of_sm(Packs, VE, false
 // Backward: one warp per (run, column tile), and behind those one per 32 table rows for the rows of
 // tokens without a run.
 template <class T, class TO, int VE, int Packs, bool Dot>
-__global__ void __launch_bounds__(kSegmentThreads, blocks_of_sm(Packs, VE, Dot))
+__global__ void __launch_bounds__(kSegmentThreads, blocks_of_sm(Packs, VE, false))
     runs_kernel(SumArgs a, SortedEntries entries, const Run* runs, const int32_t* n_runs, int64_t most_runs, const uint32_t* touched) {
     __shared__ Batch batch[kSegmentThreads / 32];
     const int64_t w = (int64_t)blockIdx.x * (kSegmentThreads / 32) + (threadIdx.x >> 5);

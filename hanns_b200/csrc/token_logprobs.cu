@@ -885,26 +885,37 @@ struct NearArgs {
     float* top_logprobs;
 };
 
-__device__ __forceinline__ double block_sum(double v, double* red) {
+// Sums over the block, N at a time; `red` has N values for each warp.
+template <int N>
+__device__ __forceinline__ void block_sums(double (&v)[N], double* red) {
 #pragma unroll
-    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    for (int d = 16; d; d >>= 1)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], d);
+    if (blockDim.x == 32) return;
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+        for (int i = 0; i < N; ++i) red[(threadIdx.x >> 5) * N + i] = v[i];
     __syncthreads();
-    v = 0.0;
-    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) v += red[w];
-    return v;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        v[i] = 0.0;
+        for (int w = 0; w < (int)(blockDim.x >> 5); ++w) v[i] += red[w * N + i];
+    }
 }
 
 // One block per row.  Everything here is f64: there are at most k + top values per row, and
 // the alternatives are ordered by sums of two sources, which f32 would tie or swap.
 template <class T>
 __global__ void __launch_bounds__(kMaxThreads) neighbours_kernel(NearArgs a) {
-    __shared__ int32_t tok[kMaxNeighbours];    // a neighbour's token, -1 where it does not count
-    __shared__ double wgt[kMaxNeighbours];     // its weight
-    __shared__ double cp[kMaxNeighbours + kMaxTop];    // candidates: log probability, token
-    __shared__ int32_t ct[kMaxNeighbours + kMaxTop];
-    __shared__ double red[kMaxThreads / 32];
+    // candidates (log probability, token), neighbours (weight; token, -1 where one does not count)
+    extern __shared__ double space[];
+    double* cp = space;
+    double* wgt = cp + a.k + a.top;
+    int32_t* ct = reinterpret_cast<int32_t*>(wgt + a.k);
+    int32_t* tok = ct + a.k + a.top;
+    __shared__ double red[3 * kMaxThreads / 32];
     __shared__ int n_cand;
     __shared__ double lp_token;  // of the given token; NaN: no neighbour's
     const int64_t r = blockIdx.x;
@@ -934,44 +945,49 @@ __global__ void __launch_bounds__(kMaxThreads) neighbours_kernel(NearArgs a) {
     __syncthreads();
     for (int w = 0; w < (int)(blockDim.x >> 5); ++w) near = fminf(near, (float)red[w]);
     if (near == INFINITY) return;  // no neighbour: the model's distribution alone
-    double sum = 0.0;
+    double sum[1] = {};
     for (int j = threadIdx.x; j < a.k; j += blockDim.x) {
         double w = 0.0;
         if (tok[j] >= 0) w = exp(((double)near - (double)a.distances[r * a.k + j]) * a.inv_tau);
         wgt[j] = w;
-        sum += w;
+        sum[0] += w;
     }
-    const double scale = a.weight / block_sum(sum, red);
+    block_sums(sum, red);
+    const double scale = a.weight / sum[0];
     const double keep = 1.0 - a.weight, log_keep = log(keep);
     // the first neighbour with a token carries the token
-    double mass = 0.0, q_log_q = 0.0, h = 0.0;
+    __syncthreads();
+    double part[3] = {};  // sums of q, q ln q, -p ln p over the neighbours' tokens
     for (int j = threadIdx.x; j < a.k; j += blockDim.x) {
         const int32_t t = tok[j];
         if (t < 0) continue;
         bool first = true;
-        for (int i = 0; i < j; ++i) first = first && tok[i] != t;
+        double w = 0.0;
+#pragma unroll 8
+        for (int i = 0; i < a.k; ++i) {
+            const bool same = tok[i] == t;
+            first = first & !(same & (i < j));
+            if (same) w += wgt[i];
+        }
         if (!first) continue;
-        double w = wgt[j];
-        for (int i = j + 1; i < a.k; ++i)
-            if (tok[i] == t) w += wgt[i];
         const double log_q = ((double)to_f32(row[t]) - m) * a.inv_t - log_s, q = exp(log_q);
         const double p = keep * q + w * scale;
-        mass += q;
-        if (q > 0.0) q_log_q += q * log_q;
+        part[0] += q;
+        if (q > 0.0) part[1] += q * log_q;
         // a probability below f64's range keeps its logarithm
         const double lp = p > 0.0 ? log(p) : log_keep + log_q;
-        if (p > 0.0) h -= p * lp;
+        if (p > 0.0) part[2] -= p * lp;
         if (t == given) lp_token = lp;
         const int at = atomicAdd(&n_cand, 1);
         cp[at] = lp;
         ct[at] = t;
     }
-    mass = block_sum(mass, red);
-    q_log_q = block_sum(q_log_q, red);
-    h = block_sum(h, red);
+    block_sums(part, red);
+    __syncthreads();
     if (threadIdx.x == 0) {
-        const double rest = fmax(1.0 - mass, 0.0);
-        if (keep > 0.0) h -= keep * (log_keep * rest - (double)st.z - q_log_q);
+        double h = part[2];
+        const double rest = fmax(1.0 - part[0], 0.0);
+        if (keep > 0.0) h -= keep * (log_keep * rest - (double)st.z - part[1]);
         a.entropy[r] = (float)fmax(h, 0.0);
         if ((uint64_t)given < (uint64_t)a.vocab) {
             double lp = lp_token;
@@ -987,7 +1003,8 @@ __global__ void __launch_bounds__(kMaxThreads) neighbours_kernel(NearArgs a) {
         const int64_t t = a.top_tokens[r * a.top + i];
         if (t < 0) continue;
         bool mine = true;
-        for (int j = 0; j < n_near; ++j) mine = mine && ct[j] != t;
+#pragma unroll 8
+        for (int j = 0; j < n_near; ++j) mine = mine & (ct[j] != t);
         if (!mine) continue;
         const int at = atomicAdd(&n_cand, 1);
         cp[at] = log_keep + ((double)to_f32(row[t]) - m) * a.inv_t - log_s;
@@ -1003,8 +1020,10 @@ __global__ void __launch_bounds__(kMaxThreads) neighbours_kernel(NearArgs a) {
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
         const double lp = cp[i];
         if (!(lp > -INFINITY)) continue;
+        const int32_t t = ct[i];
         int rank = 0;
-        for (int j = 0; j < n; ++j) rank += cp[j] > lp || (cp[j] == lp && ct[j] < ct[i]);
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) rank += (cp[j] > lp) | ((cp[j] == lp) & (ct[j] < t));
         if (rank < a.top) {
             a.top_tokens[r * a.top + rank] = ct[i];
             a.top_logprobs[r * a.top + rank] = (float)lp;
@@ -1176,10 +1195,11 @@ extern "C" int32_t hanns_gpu_neighbour_logprobs_device(const hanns_token_logprob
         a.top_tokens = t->top_tokens;
         a.top_logprobs = t->top_logprobs;
         cudaStream_t s = static_cast<cudaStream_t>(stream);
-        const unsigned threads = k <= 32 ? 32 : k <= 128 ? 128 : kMaxThreads;
-        if (t->dtype == HANNS_DTYPE_F32) neighbours_kernel<float><<<(unsigned)t->n, threads, 0, s>>>(a);
-        else if (t->dtype == HANNS_DTYPE_F16) neighbours_kernel<__half><<<(unsigned)t->n, threads, 0, s>>>(a);
-        else neighbours_kernel<__nv_bfloat16><<<(unsigned)t->n, threads, 0, s>>>(a);
+        const unsigned threads = k <= 32 ? 32 : k <= 64 ? 64 : kMaxThreads, n = (unsigned)t->n;
+        const size_t shared = (2 * (size_t)k + a.top) * sizeof(double) + (2 * (size_t)k + a.top) * sizeof(int32_t);
+        if (t->dtype == HANNS_DTYPE_F32) neighbours_kernel<float><<<n, threads, shared, s>>>(a);
+        else if (t->dtype == HANNS_DTYPE_F16) neighbours_kernel<__half><<<n, threads, shared, s>>>(a);
+        else neighbours_kernel<__nv_bfloat16><<<n, threads, shared, s>>>(a);
         HANNS_CUDA_OK(cudaGetLastError());
     });
 }
