@@ -766,6 +766,125 @@ __global__ void __launch_bounds__(kThreads) sort_runs_kernel(SortArgs a, const u
     if (begins) a.runs[at] = Run{(int32_t)k, (int32_t)i, (int32_t)end, 0};
 }
 
+// The whole sort and the list of runs for up to kSmallSort positions: one block, the keys in shared
+// memory, instead of seven launches whose work is nothing beside their starts.
+constexpr int kSmallThreads = 1024, kSmallWarps = kSmallThreads / 32, kSmallItems = 4;
+constexpr int kSmallSort = kSmallThreads * kSmallItems, kSmallBits = 8;
+constexpr int64_t kSmallRows = 1 << 20;  // bit maps that one block clears quickly
+
+__global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(SortArgs a, int passes) {
+    __shared__ uint32_t s_key[kSmallSort];
+    __shared__ uint16_t s_pos[kSmallSort];
+    __shared__ uint16_t seen[kSmallWarps][1 << kSmallBits];  // a warp's keys per digit, then its first place
+    __shared__ int32_t warp_sum[(1 << kSmallBits) / 32];
+    __shared__ int32_t n_runs;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (threadIdx.x < 2) a.list_counts[threadIdx.x] = 0;
+    if (threadIdx.x == 0) n_runs = 0;
+    for (int64_t i = threadIdx.x; i < (a.rows + 31) / 32; i += kSmallThreads) a.touched[i] = a.lengthy[i] = 0;
+    uint32_t key[kSmallItems];
+    uint16_t pos[kSmallItems];
+    // places of this thread's items, in every pass
+    auto place = [&](int i) { return warp * (32 * kSmallItems) + i * 32 + lane; };
+#pragma unroll
+    for (int i = 0; i < kSmallItems; ++i) {
+        const int j = place(i);
+        pos[i] = (uint16_t)j;
+        key[i] = 0xffffffffu;  // behind the last position
+        if (j >= a.n) continue;
+        const int64_t t = a.tokens[j];
+        int32_t bag = -1;
+        if ((uint64_t)t < (uint64_t)a.rows) {
+            const int64_t starts = a.bags.offsets ? a.bags.starts_up_to(j) : j + 1;
+            if (starts <= a.bags.n_bags) bag = (int32_t)starts - 1;
+        }
+        a.bag[j] = bag;
+        key[i] = bag >= 0 ? (uint32_t)t : (uint32_t)a.rows;
+    }
+    for (int p = 0; p < passes; ++p) {
+        const int shift = p * kSmallBits;
+        for (int b = threadIdx.x; b < kSmallWarps << (kSmallBits - 1); b += kSmallThreads) reinterpret_cast<uint32_t*>(&seen[0][0])[b] = 0;
+        __syncthreads();
+        int rank[kSmallItems];
+#pragma unroll
+        for (int i = 0; i < kSmallItems; ++i) {
+            const int d = (key[i] >> shift) & ((1 << kSmallBits) - 1);
+            const uint32_t peers = __match_any_sync(0xffffffffu, d);
+            rank[i] = seen[warp][d] + __popc(peers & ((1u << lane) - 1));
+            __syncwarp();
+            if ((peers >> lane) == 1) seen[warp][d] += (uint16_t)__popc(peers);
+            __syncwarp();
+        }
+        __syncthreads();
+        int32_t total = 0, upto = 0;
+        if (threadIdx.x < 1 << kSmallBits) {
+            for (int w = 0; w < kSmallWarps; ++w) {
+                const int c = seen[w][threadIdx.x];
+                seen[w][threadIdx.x] = (uint16_t)total;
+                total += c;
+            }
+            upto = total;
+#pragma unroll
+            for (int m = 1; m < 32; m <<= 1) {
+                const int32_t o = __shfl_up_sync(0xffffffffu, upto, m);
+                if (lane >= m) upto += o;
+            }
+            if (lane == 31) warp_sum[warp] = upto;
+        }
+        __syncthreads();
+        if (threadIdx.x < 1 << kSmallBits) {
+            int32_t before = upto - total;
+            for (int w = 0; w < warp; ++w) before += warp_sum[w];
+            for (int w = 0; w < kSmallWarps; ++w) seen[w][threadIdx.x] += (uint16_t)before;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kSmallItems; ++i) {
+            const int to = seen[warp][(key[i] >> shift) & ((1 << kSmallBits) - 1)] + rank[i];
+            s_key[to] = key[i];
+            s_pos[to] = pos[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kSmallItems; ++i) {
+            key[i] = s_key[place(i)];
+            pos[i] = s_pos[place(i)];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kSmallItems; ++i) {
+        const int at = place(i);
+        const uint32_t k = key[i];
+        const bool begins = k < a.rows && (at == 0 || s_key[at - 1] != k);
+        if (at < a.n) {
+            const int32_t bag = a.bag[pos[i]];
+            a.pos_out[at] = pos[i];
+            a.src[at] = bag;
+            a.coef[at] = entry_factor(a, pos[i], bag);
+        }
+        int end = at + 1;
+        if (begins) {
+            int in = at, step = 1;  // s_key[in] is k
+            while (in + step < a.n && s_key[in + step] == k) {
+                in += step;
+                step *= 2;
+            }
+            for (; step; step >>= 1)
+                if (in + step < a.n && s_key[in + step] == k) in += step;
+            end = in + 1;
+            atomicOr(a.touched + k / 32, 1u << (k & 31));
+            if (end - at > kLimit) atomicOr(a.lengthy + k / 32, 1u << (k & 31));
+        }
+        const uint32_t who = __ballot_sync(0xffffffffu, begins);
+        int32_t to = 0;
+        if (lane == 0 && who) to = atomicAdd(&n_runs, __popc(who));
+        to = __shfl_sync(0xffffffffu, to, 0) + __popc(who & ((1u << lane) - 1));
+        if (begins) a.runs[to] = Run{(int32_t)k, at, end, 0};
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) *a.n_runs = n_runs;
+}
+
 // dw_j: the column tiles' inner products in order, times scale / c_bag; 0 where j does not count.
 __global__ void __launch_bounds__(kThreads) weights_grad_kernel(const float* dot, int tiles, int piece_tiles, SortArgs a, float* d_weights) {
     const int64_t j = (int64_t)blockIdx.x * kThreads + threadIdx.x;
@@ -1095,6 +1214,13 @@ extern "C" int32_t hanns_gpu_embed_bags_grad_device(const hanns_embed_bags_t* b,
         if (n == 0) {
             HANNS_CUDA_OK(cudaMemsetAsync(so.touched, 0, (b->rows + 31) / 32 * sizeof(uint32_t), s));
             HANNS_CUDA_OK(cudaMemsetAsync(so.n_runs, 0, sizeof(int32_t), s));
+        } else if (n <= kSmallSort && b->rows <= kSmallRows) {
+            int passes = 1;
+            while (b->rows >> (passes * kSmallBits)) ++passes;  // keys 0 .. rows
+            so.pos_out = gs.pos[0];
+            position = so.pos_out;
+            sort_small_kernel<<<1, kSmallThreads, 0, s>>>(so, passes);
+            HANNS_CUDA_OK(cudaGetLastError());
         } else {
             for (int p = 0; p < sp.passes; ++p) {
                 so.shift = p * sp.bits;

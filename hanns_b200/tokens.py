@@ -35,21 +35,28 @@ def _need(ok, what: str):
         raise ValueError(what)
 
 
-def _on(t, device, name):
-    _need(isinstance(t, torch.Tensor), f"{name} must be a tensor")
-    _need(t.device == device, f"{name} must be on {device}, not {t.device}")
-
-
+# (messages are put together only when they are raised: these run on every call)
 def _cuda(t, name):
-    _need(isinstance(t, torch.Tensor), f"{name} must be a tensor")
-    _need(t.dtype in _DTYPES, f"{name} must be float32, float16 or bfloat16, not {t.dtype}")
-    _need(t.is_cuda, f"{name} must be on a CUDA device, not {t.device}")
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a tensor")
+    if t.dtype not in _DTYPES:
+        raise ValueError(f"{name} must be float32, float16 or bfloat16, not {t.dtype}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on a CUDA device, not {t.device}")
+
+
+def _on(t, device, name):
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a tensor")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, not {t.device}")
 
 
 def _ids(t, device, name):
     _on(t, device, name)
     if t.dtype != torch.int64:
-        _need(t.dtype == torch.int32, f"{name} must be int64 or int32, not {t.dtype}")
+        if t.dtype != torch.int32:
+            raise ValueError(f"{name} must be int64 or int32, not {t.dtype}")
         t = t.to(torch.int64)
     return t if t.is_contiguous() else t.contiguous()
 
@@ -79,6 +86,12 @@ def _workspace(nbytes, device, b):
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     b.workspace, b.workspace_bytes = ws.data_ptr(), nbytes
     return ws
+
+
+def _once(what):
+    """Gradients are enabled in a backward pass only where it is to be differentiated itself."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} can be differentiated once only")
 
 
 # ---------------------------------------------------------------------------- embed_bags
@@ -117,8 +130,8 @@ class _EmbedBags(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        _once("embed_bags")
         d_table, d_weights = _embed_bags_grad(grad, *ctx.saved_tensors, *ctx.args,
                                               ctx.needs_input_grad[0], ctx.needs_input_grad[3])
         return d_table, None, None, d_weights, None, None, None
@@ -167,7 +180,7 @@ def embed_bags(table, tokens, offsets=None, weights=None, *, scale: float = 1.0,
     _need(table.dim() == 2 and table.shape[0] > 0 and table.shape[1] > 0, "table must be [rows, dim]")
     dev = table.device
     out_dtype = out_dtype or table.dtype
-    _need(out_dtype in (table.dtype, torch.float32), "out_dtype must be the table's type or float32")
+    _need(out_dtype is torch.float32 or out_dtype is table.dtype, "out_dtype must be the table's type or float32")
     tokens = _ids(tokens, dev, "tokens")
     shape = tokens.shape
     if offsets is None:
@@ -250,23 +263,33 @@ def _token_logprobs(logits, tokens, top, temperature, near, keep):
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top, temperature):
-        out = _token_logprobs(logits, tokens, top, temperature, None, True)
-        ctx.mark_non_differentiable(out[2])
+        lp, h, tt, tl, ctx.stats = _token_logprobs(logits, tokens, top, temperature, None, True)
+        ctx.mark_non_differentiable(tt)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, tokens, *out)
+        ctx.save_for_backward(logits, tokens, tt)
         ctx.args = top, temperature
-        return out[:4]
+        return lp, h, tt, tl
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_logprobs, g_entropy, _, g_top):
-        logits, tokens, *out = ctx.saved_tensors
-        dev = logits.device
-        g = [None if x is None else x.to(torch.float32).contiguous() for x in (g_logprobs, g_entropy, g_top)]
-        d = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-        t = _probs(logits, tokens, *ctx.args, out)
-        _run(dev, lambda stream: _check(L.lib().hanns_gpu_token_logprobs_grad_device(
-            C.byref(t), *(_ptr(x) for x in g), d.data_ptr(), logits.shape[1], stream), "token_logprobs"))
+        _once("token_logprobs")
+        logits, tokens, tt = ctx.saved_tensors
+        top, temperature = ctx.args
+        if g_logprobs is not None:
+            g_logprobs = g_logprobs.contiguous()
+        if g_entropy is not None:
+            g_entropy = g_entropy.contiguous()
+        if g_top is not None:
+            g_top = g_top.contiguous()
+        d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        n, vocab = logits.shape
+        # the forward call's outputs are not read: any non-null pointer stands for them
+        ptr = logits.data_ptr()
+        t = L.TokenLogprobs(_DTYPES[logits.dtype], top, n, vocab, logits.stride(0), temperature, 0, ptr,
+                            tokens.data_ptr(), ptr, ptr, tt.data_ptr(), ptr, ctx.stats.data_ptr())
+        _run(logits.device, lambda stream: _check(L.lib().hanns_gpu_token_logprobs_grad_device(
+            C.byref(t), _ptr(g_logprobs), _ptr(g_entropy), _ptr(g_top), d.data_ptr(), vocab, stream),
+            "token_logprobs"))
         return d, None, None, None
 
 
