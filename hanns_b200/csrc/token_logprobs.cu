@@ -440,36 +440,23 @@ __device__ __forceinline__ void write_row(const ProbArgs& a, int64_t r, int64_t 
     }
 }
 
-template <class T, bool Top>
-__global__ void __launch_bounds__(kMaxThreads, 8) logprobs_kernel(ProbArgs a) {
-    constexpr int VE = RowView<T>::VE;
-    __shared__ Shared sh;
-    cg::cluster_group cluster = cg::this_cluster();
-    const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
-    const int64_t r = blockIdx.x / parts;
-    const T* row = static_cast<const T*>(a.logits) + r * a.ld;
-    const RowView<T> view(row, a.vocab);
-    const int nvec = view.vectors(), per = (nvec + parts - 1) / parts;
-    const int v0 = min(nvec, part * per), v1 = min(nvec, v0 + per);
-    int64_t token = -1;
-    float x_t = 0.0f;
-    if (part == 0 && threadIdx.x == 0) {
-        token = a.tokens[r];
-        if ((uint64_t)token < (uint64_t)a.vocab) x_t = to_f32(row[token]);
+// A block's share of a row: vectors [v0, v1), of them [b0, b1) of the body.
+template <class T>
+struct Columns {
+    RowView<T> view;
+    int v0, v1, b0, b1;
+    __device__ __forceinline__ Columns(const ProbArgs& a, int64_t r, int part, int parts)
+        : view(static_cast<const T*>(a.logits) + r * a.ld, a.vocab) {
+        const int nvec = view.vectors(), per = (nvec + parts - 1) / parts;
+        v0 = min(nvec, part * per);
+        v1 = min(nvec, v0 + per);
+        b0 = max(0, v0 - view.skipped());
+        b1 = min(view.n, v1 - view.skipped());
     }
-    if (threadIdx.x == 0) sh.count = 0;
-
-    Running<T> run(a.c);
-    float best = -INFINITY, second = -INFINITY, third = -INFINITY;  // largest maxima of this thread's rounds
-    int best_round = 0, second_round = 0;
-    const int step = blockDim.x * kUnroll;
-    // this block's vectors of the body, in rounds of kUnroll per thread
-    const int b0 = max(0, v0 - view.skipped()), b1 = min(view.n, v1 - view.skipped());
-    int round = 0;
-    for (int base = b0; base < b1; base += step, ++round) {
-        Pack<T, VE> p[kUnroll];
-        const Pack<T, VE>* src = view.body + base + threadIdx.x;
-        if (base + step <= b1) {
+    // a round of kUnroll vectors per thread, -inf behind the last
+    __device__ __forceinline__ void fetch(int base, Pack<T, RowView<T>::VE> (&p)[kUnroll]) const {
+        const Pack<T, RowView<T>::VE>* src = view.body + base + threadIdx.x;
+        if (base + (int)blockDim.x * kUnroll <= b1) {
 #pragma unroll
             for (int q = 0; q < kUnroll; ++q) p[q] = src[q * blockDim.x];
         } else {
@@ -479,169 +466,213 @@ __global__ void __launch_bounds__(kMaxThreads, 8) logprobs_kernel(ProbArgs a) {
                     p[q] = src[q * blockDim.x];
                 } else {
 #pragma unroll
-                    for (int k = 0; k < VE; ++k) p[q].v[k] = from_f32<T>(-INFINITY);
+                    for (int k = 0; k < RowView<T>::VE; ++k) p[q].v[k] = from_f32<T>(-INFINITY);
                 }
             }
         }
-        const float vm = packs_max(p);
-        if (Top) {
-            third = fmaxf(third, fminf(second, vm));
-            if (vm > second) {
-                const bool first = vm > best;
-                second = first ? best : vm;
-                second_round = first ? best_round : round;
-                best = first ? vm : best;
-                best_round = first ? round : best_round;
-            }
-        }
-        run.reach(vm, a.c);
-#pragma unroll
-        for (int q = 0; q < kUnroll; ++q) run.add(p[q], a.c);
     }
-    // the alternatives' candidates: a thread whose maxima reach the threshold reads those rounds
-    // again; where a third one does, its warp reads all of that thread's rounds
-    float thr = -INFINITY;
-    if (Top) {
-        thr = block_threshold(sh, best, a.top);
-        auto offer_vector = [&](int j) {
-            const float pm = pack_max(view.body[j]);
-            if (pm >= thr && pm > -INFINITY) sh.choice().offer(cand_key(pm, view.skipped() + j));
-        };
-        const bool many = third >= thr && third > -INFINITY;
-        if (!many) {
-            for (int k = 0; k < 2; ++k) {
-                if ((k ? second : best) < thr || (k ? second : best) == -INFINITY) break;
-                const int j = b0 + (k ? second_round : best_round) * step + (int)threadIdx.x;
-#pragma unroll
-                for (int q = 0; q < kUnroll; ++q)
-                    if (j + q * (int)blockDim.x < b1) offer_vector(j + q * (int)blockDim.x);
-            }
-        }
-        for (uint32_t who = __ballot_sync(0xffffffffu, many); who; who &= who - 1) {
-            const int j0 = b0 + (int)(threadIdx.x & ~31u) + __ffs(who) - 1;
-            for (int j = j0 + (int)(threadIdx.x & 31) * (int)blockDim.x; j < b1; j += 32 * (int)blockDim.x) offer_vector(j);
-        }
-    }
-    // the partial vectors at the row's ends
-    if (threadIdx.x < 2) {
-        const int i = threadIdx.x ? view.skipped() + view.n : 0;
-        if ((threadIdx.x || view.skipped()) && i >= v0 && i < v1) {
-            const Pack<T, VE> p = view.edge(i);
-            const float vm = pack_max(p);
-            if (Top && vm >= thr && vm > -INFINITY) sh.choice().offer(cand_key(vm, i));
-            run.reach(vm, a.c);
-            run.add(p, a.c);
-        }
-    }
+};
 
-    // the warp's sums against its largest reference, then the block's
-    float m = run.m, ref = run.ref, s = run.s.x + run.s.y, u = run.u.x + run.u.y;
-#pragma unroll
-    for (int d = 16; d; d >>= 1) {
-        m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
-        ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, d));
-    }
-    rescale(run.ref - ref, s, u);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) {
-        s += __shfl_xor_sync(0xffffffffu, s, d);
-        u += __shfl_xor_sync(0xffffffffu, u, d);
-    }
-    const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    if ((threadIdx.x & 31) == 0) {
-        sh.wm[warp] = m;
-        sh.wr[warp] = ref;
-        sh.ws[warp] = s;
-        sh.wu[warp] = u;
-    }
-    __syncthreads();
-    m = sh.wm[0];
-    ref = sh.wr[0];
-    for (int w = 1; w < warps; ++w) {
-        m = max_nan(m, sh.wm[w]);
-        ref = fmaxf(ref, sh.wr[w]);
-    }
-    s = u = 0.0f;
-    for (int w = 0; w < warps; ++w) {
-        float ps = sh.ws[w], pu = sh.wu[w];
-        rescale(sh.wr[w] - ref, ps, pu);
-        s += ps;
-        u += pu;
-    }
-    if (threadIdx.x == 0) {
-        sh.m = m;
-        sh.ref = ref;
-        sh.s = s;
-        sh.u = u;
-    }
-    if (Top) {
-        if (sh.count > kCap) select_again(sh, view, v0, v1, a.top);
-        else select_elements<BlockGroup>(sh.choice(), view, a.top);
-    }
-    if (parts > 1) {
-        cluster.sync();
-        for (int q = 0; q < parts; ++q) {
-            const Shared* o = cluster.map_shared_rank(&sh, q);
-            m = q ? max_nan(m, o->m) : o->m;
-            ref = q ? fmaxf(ref, o->ref) : o->ref;
+// Without alternatives a block takes a row after the other, and the first round of the next one is
+// on the way while a row is brought to its end (4096 x 128,000 bf16: 176 -> 174 us, 4099 x 50,257:
+// 80 -> 77).  With them it takes one: their second look at the row would wait behind that round
+// (with 5 alternatives: 93 -> 107 us).
+template <class T, bool Top>
+__global__ void __launch_bounds__(kMaxThreads, 8) logprobs_kernel(ProbArgs a, int64_t n) {
+    constexpr int VE = RowView<T>::VE;
+    __shared__ Shared sh;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
+    int64_t r = blockIdx.x / parts;
+    Columns<T> c(a, r, part, parts);
+    Pack<T, VE> p[kUnroll];
+    c.fetch(c.b0, p);
+    while (true) {
+        const RowView<T>& view = c.view;
+        const T* row = view.row;
+        const int v0 = c.v0, v1 = c.v1, b0 = c.b0, b1 = c.b1;
+        int64_t token = -1;
+        float x_t = 0.0f;
+        if (part == 0 && threadIdx.x == 0) {
+            token = a.tokens[r];
+            if ((uint64_t)token < (uint64_t)a.vocab) x_t = to_f32(row[token]);
         }
-    }
-    const bool empty = m == -INFINITY, undefined = !(m < INFINITY);
-    const bool differences = !empty && !undefined && row_needs_differences<T>(m, a.c);
-    if (differences) {
-        s = u = 0.0f;
-        const int64_t e1 = min((int64_t)a.vocab, view.first(v1));
-        for (int64_t e = max((int64_t)0, view.first(v0)) + threadIdx.x; e < e1; e += blockDim.x) {
-            const float y = fmaxf((to_f32(row[e]) - m) * a.c, kLowest), f = ex2(y);
-            s += f;
-            u = fmaf(f, y, u);
+        if (threadIdx.x == 0) sh.count = 0;
+
+        Running<T> run(a.c);
+        float best = -INFINITY, second = -INFINITY, third = -INFINITY;  // largest maxima of this thread's rounds
+        int best_round = 0, second_round = 0;
+        const int step = blockDim.x * kUnroll;
+        int round = 0;
+        for (int base = b0; base < b1; base += step, ++round) {
+            if (round) c.fetch(base, p);
+            const float vm = packs_max(p);
+            if (Top) {
+                third = fmaxf(third, fminf(second, vm));
+                if (vm > second) {
+                    const bool first = vm > best;
+                    second = first ? best : vm;
+                    second_round = first ? best_round : round;
+                    best = first ? vm : best;
+                    best_round = first ? round : best_round;
+                }
+            }
+            run.reach(vm, a.c);
+#pragma unroll
+            for (int q = 0; q < kUnroll; ++q) run.add(p[q], a.c);
         }
+        const int64_t next_r = r + gridDim.x / parts;
+        const Columns<T> next(a, min(next_r, n - 1), part, parts);
+        if (!Top && next_r < n) next.fetch(next.b0, p);
+        // the alternatives' candidates: a thread whose maxima reach the threshold reads those rounds
+        // again; where a third one does, its warp reads all of that thread's rounds
+        float thr = -INFINITY;
+        if (Top) {
+            thr = block_threshold(sh, best, a.top);
+            auto offer_vector = [&](int j) {
+                const float pm = pack_max(view.body[j]);
+                if (pm >= thr && pm > -INFINITY) sh.choice().offer(cand_key(pm, view.skipped() + j));
+            };
+            const bool many = third >= thr && third > -INFINITY;
+            if (!many) {
+                for (int k = 0; k < 2; ++k) {
+                    if ((k ? second : best) < thr || (k ? second : best) == -INFINITY) break;
+                    const int j = b0 + (k ? second_round : best_round) * step + (int)threadIdx.x;
+#pragma unroll
+                    for (int q = 0; q < kUnroll; ++q)
+                        if (j + q * (int)blockDim.x < b1) offer_vector(j + q * (int)blockDim.x);
+                }
+            }
+            for (uint32_t who = __ballot_sync(0xffffffffu, many); who; who &= who - 1) {
+                const int j0 = b0 + (int)(threadIdx.x & ~31u) + __ffs(who) - 1;
+                for (int j = j0 + (int)(threadIdx.x & 31) * (int)blockDim.x; j < b1; j += 32 * (int)blockDim.x) offer_vector(j);
+            }
+        }
+        // the partial vectors at the row's ends
+        if (threadIdx.x < 2) {
+            const int i = threadIdx.x ? view.skipped() + view.n : 0;
+            if ((threadIdx.x || view.skipped()) && i >= v0 && i < v1) {
+                const Pack<T, VE> p = view.edge(i);
+                const float vm = pack_max(p);
+                if (Top && vm >= thr && vm > -INFINITY) sh.choice().offer(cand_key(vm, i));
+                run.reach(vm, a.c);
+                run.add(p, a.c);
+            }
+        }
+
+        // the warp's sums against its largest reference, then the block's
+        float m = run.m, ref = run.ref, s = run.s.x + run.s.y, u = run.u.x + run.u.y;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+            m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+            ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, d));
+        }
+        rescale(run.ref - ref, s, u);
 #pragma unroll
         for (int d = 16; d; d >>= 1) {
             s += __shfl_xor_sync(0xffffffffu, s, d);
             u += __shfl_xor_sync(0xffffffffu, u, d);
         }
-        __syncthreads();
+        const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
         if ((threadIdx.x & 31) == 0) {
+            sh.wm[warp] = m;
+            sh.wr[warp] = ref;
             sh.ws[warp] = s;
             sh.wu[warp] = u;
         }
         __syncthreads();
+        m = sh.wm[0];
+        ref = sh.wr[0];
+        for (int w = 1; w < warps; ++w) {
+            m = max_nan(m, sh.wm[w]);
+            ref = fmaxf(ref, sh.wr[w]);
+        }
         s = u = 0.0f;
         for (int w = 0; w < warps; ++w) {
-            s += sh.ws[w];
-            u += sh.wu[w];
+            float ps = sh.ws[w], pu = sh.wu[w];
+            rescale(sh.wr[w] - ref, ps, pu);
+            s += ps;
+            u += pu;
         }
         if (threadIdx.x == 0) {
+            sh.m = m;
+            sh.ref = ref;
             sh.s = s;
             sh.u = u;
         }
-        if (parts > 1) cluster.sync();
-    }
-    if (part == 0) {
+        if (Top) {
+            if (sh.count > kCap) select_again(sh, view, v0, v1, a.top);
+            else select_elements<BlockGroup>(sh.choice(), view, a.top);
+        }
         if (parts > 1) {
-            s = u = 0.0f;
+            cluster.sync();
             for (int q = 0; q < parts; ++q) {
                 const Shared* o = cluster.map_shared_rank(&sh, q);
-                float ps = o->s, pu = o->u;
-                if (!differences) rescale(o->ref - ref, ps, pu);
-                s += ps;
-                u += pu;
-            }
-            if (Top) {
-                if (threadIdx.x == 0) sh.count = 0;
-                __syncthreads();
-                for (int i = threadIdx.x; i < parts * a.top; i += blockDim.x) {
-                    const uint64_t k = cluster.map_shared_rank(&sh, i / a.top)->best[i % a.top];
-                    if (k) sh.elem[atomicAdd(&sh.count, 1)] = k;
-                }
-                __syncthreads();
-                rank_select<BlockGroup>(sh.elem, sh.count, sh.best, a.top);
+                m = q ? max_nan(m, o->m) : o->m;
+                ref = q ? fmaxf(ref, o->ref) : o->ref;
             }
         }
-        write_row<BlockGroup>(a, r, token, x_t, m, ref, s, u, differences, sh.best);
+        const bool empty = m == -INFINITY, undefined = !(m < INFINITY);
+        const bool differences = !empty && !undefined && row_needs_differences<T>(m, a.c);
+        if (differences) {
+            s = u = 0.0f;
+            const int64_t e1 = min((int64_t)a.vocab, view.first(v1));
+            for (int64_t e = max((int64_t)0, view.first(v0)) + threadIdx.x; e < e1; e += blockDim.x) {
+                const float y = fmaxf((to_f32(row[e]) - m) * a.c, kLowest), f = ex2(y);
+                s += f;
+                u = fmaf(f, y, u);
+            }
+#pragma unroll
+            for (int d = 16; d; d >>= 1) {
+                s += __shfl_xor_sync(0xffffffffu, s, d);
+                u += __shfl_xor_sync(0xffffffffu, u, d);
+            }
+            __syncthreads();
+            if ((threadIdx.x & 31) == 0) {
+                sh.ws[warp] = s;
+                sh.wu[warp] = u;
+            }
+            __syncthreads();
+            s = u = 0.0f;
+            for (int w = 0; w < warps; ++w) {
+                s += sh.ws[w];
+                u += sh.wu[w];
+            }
+            if (threadIdx.x == 0) {
+                sh.s = s;
+                sh.u = u;
+            }
+            if (parts > 1) cluster.sync();
+        }
+        if (part == 0) {
+            if (parts > 1) {
+                s = u = 0.0f;
+                for (int q = 0; q < parts; ++q) {
+                    const Shared* o = cluster.map_shared_rank(&sh, q);
+                    float ps = o->s, pu = o->u;
+                    if (!differences) rescale(o->ref - ref, ps, pu);
+                    s += ps;
+                    u += pu;
+                }
+                if (Top) {
+                    if (threadIdx.x == 0) sh.count = 0;
+                    __syncthreads();
+                    for (int i = threadIdx.x; i < parts * a.top; i += blockDim.x) {
+                        const uint64_t k = cluster.map_shared_rank(&sh, i / a.top)->best[i % a.top];
+                        if (k) sh.elem[atomicAdd(&sh.count, 1)] = k;
+                    }
+                    __syncthreads();
+                    rank_select<BlockGroup>(sh.elem, sh.count, sh.best, a.top);
+                }
+            }
+            write_row<BlockGroup>(a, r, token, x_t, m, ref, s, u, differences, sh.best);
+        }
+        if (parts > 1) cluster.sync();  // the others' shared memory stays until it has been read
+        if (Top || next_r >= n) break;
+        __syncthreads();
+        r = next_r;
+        c = next;
     }
-    if (parts > 1) cluster.sync();  // the others' shared memory stays until it has been read
 }
 
 // Short rows: a warp takes a row whose vectors (the partial ones among them) fit in its
@@ -1066,7 +1097,8 @@ void launch_probs(const hanns_token_logprobs_t* t, const ProbArgs& a, cudaStream
     while (parts < kMaxCluster && t->n * parts * 2 <= want && vectors / (parts * 2) >= kMaxThreads * kUnroll) parts *= 2;
     const int threads = kMaxThreads;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(t->n * parts));
+    // blocks that take several rows: as many as are resident
+    cfg.gridDim = dim3((unsigned)(Top || parts > 1 ? t->n * parts : std::min<int64_t>(t->n, 8 * sm_count())));
     cfg.blockDim = dim3((unsigned)threads);
     cfg.stream = s;
     cudaLaunchAttribute at[1];
@@ -1074,7 +1106,7 @@ void launch_probs(const hanns_token_logprobs_t* t, const ProbArgs& a, cudaStream
     at[0].val.clusterDim = {(unsigned)parts, 1, 1};
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    HANNS_CUDA_OK(cudaLaunchKernelEx(&cfg, logprobs_kernel<T, Top>, a));
+    HANNS_CUDA_OK(cudaLaunchKernelEx(&cfg, logprobs_kernel<T, Top>, a, t->n));
 }
 
 template <class T>
