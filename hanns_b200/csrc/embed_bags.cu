@@ -40,8 +40,8 @@ constexpr int kDots = 8;              // inner products that are reduced togethe
 // that its registers are kept to (more spill, fewer leave the memory idle).
 constexpr int kMostPacks = 4;
 __host__ __device__ constexpr int rows_ahead(int packs) { return packs == 1 ? 8 : packs == 2 ? 3 : 2; }
-constexpr int blocks_of_sm(int packs, int ve, bool forward) { return packs == 1 ? 14 : forward ? (ve == 8 ? 16 : 18) : ve == 8 ? 10 : 14; }
-constexpr int kLookupRows = 8;        // rows of a warp in a lookup
+constexpr int blocks_of_sm(int packs, int ve, bool forward) { return packs == 1 ? 14 : ve == 1 ? 16 : forward ? (ve == 8 ? 16 : 18) : ve == 8 ? 10 : 14; }
+constexpr int kLookupPacks = 8;       // vectors of a lane in a lookup
 constexpr int kMaxBinBits = 9, kMaxBins = 1 << kMaxBinBits;
 constexpr int kSortItems = 4, kSortTile = kThreads * kSortItems;
 
@@ -76,14 +76,9 @@ __device__ __forceinline__ int64_t clamp_pos(int64_t p, int64_t lo, int64_t hi) 
 
 // Bags: [offsets[i], offsets[i+1]), kept inside [0, n_tokens] whatever the offsets hold.
 struct BagSegments {
-    const int64_t* offsets;  // null: bag i is position i
+    const int64_t* offsets;  // null: bag i is position i, and the functions here are not called
     int64_t n_bags, n_tokens;
     __device__ __forceinline__ void bounds(int64_t i, int64_t& lo, int64_t& hi) const {
-        if (!offsets) {
-            lo = i;
-            hi = i + 1;
-            return;
-        }
         lo = clamp_pos(offsets[i], 0, n_tokens);
         hi = clamp_pos(offsets[i + 1], lo, n_tokens);
     }
@@ -215,11 +210,8 @@ struct Batch {
     int32_t pos[32];
 };
 
-template <int VE, int Packs>
-using Sums = float2[Packs][(VE + 1) / 2];
-
-// Entries q, q + groups, ... of a batch of n, N per group (all there when Full).  from[t]: vector
-// t of the matrix's first row; vectors behind the row's end are the last one's again.
+// Entries q, q + groups, ... of a batch of n, N per group (all there when Full).  step[t]: column of
+// vector t; vectors behind the row's end are the first one's again.
 template <class T, int VE, int Packs, bool Dot, int N, bool Full>
 __device__ __forceinline__ void add_rows(const SumArgs& a, const Lanes& ln, const Batch& bt, const char* base, const int (&step)[Packs],
                                          int q, int n, float2 (&acc)[Packs][(VE + 1) / 2], const float2 (&e)[Packs][(VE + 1) / 2],
@@ -493,40 +485,49 @@ __global__ void __launch_bounds__(kSegmentThreads, Dot ? 12 : 14) pieces_kernel(
     }
 }
 
-// Bags of one token: a warp moves a column tile of kLookupRows rows.
-template <class T, class TO, int VE>
+// Bags of one token: a warp moves a column tile of several rows, kLookupPacks vectors a lane in all.
+template <class T, class TO, int VE, int Packs>
 __global__ void __launch_bounds__(kSegmentThreads) lookup_kernel(SumArgs a, TokenEntries entries) {
+    constexpr int kRows = kLookupPacks / Packs, H = (VE + 1) / 2;
     const uint32_t w = blockIdx.x * (kSegmentThreads / 32) + (threadIdx.x >> 5);
     const uint32_t batch = w / (uint32_t)a.tiles, tile = w - batch * (uint32_t)a.tiles;
-    const Lanes ln(a, tile, VE, 1);
-    const int64_t first = (int64_t)batch * kLookupRows * ln.groups;
+    const Lanes ln(a, tile, VE, Packs);
+    const int64_t first = (int64_t)batch * kRows * ln.groups;
     if (first >= a.n_segments) return;
-    const T* base = static_cast<const T*>(a.base) + ln.col;
-    Pack<T, VE> p[kLookupRows];
-    int row[kLookupRows];
-    float f[kLookupRows];
+    const T* base = static_cast<const T*>(a.base);
+    Pack<T, VE> p[kRows][Packs];
+    int row[kRows];
+    float f[kRows];
 #pragma unroll
-    for (int u = 0; u < kLookupRows; ++u) {
+    for (int u = 0; u < kRows; ++u) {
         const int64_t i = first + u * ln.groups + ln.group;
         row[u] = -1;
         f[u] = 0.0f;
         if (i < a.n_segments) entries.get(i, row[u], f[u]);
     }
 #pragma unroll
-    for (int u = 0; u < kLookupRows; ++u)
-        if (row[u] >= 0 && ln.col < a.dim) p[u] = load_pack<T, VE>(base + (int64_t)row[u] * a.ld);
+    for (int u = 0; u < kRows; ++u)
 #pragma unroll
-    for (int u = 0; u < kLookupRows; ++u) {
+        for (int t = 0; t < Packs; ++t)
+            if (row[u] >= 0 && ln.col + t * 32 * VE < a.dim)
+                p[u][t] = load_pack<T, VE>(base + (int64_t)row[u] * a.ld + ln.col + t * 32 * VE);
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
         const int64_t i = first + u * ln.groups + ln.group;
         if (i >= a.n_segments) continue;
-        float2 acc[(VE + 1) / 2] = {};
-        if (row[u] >= 0 && ln.col < a.dim) {
-            unpack(p[u], acc);
-#pragma unroll
-            for (int k = 0; k < (VE + 1) / 2; ++k) acc[k] = mul2_rn(acc[k], make_float2(f[u], f[u]));
-        }
         if (a.mean && a.inv_counts && tile == 0 && (ln.lane & (ln.count - 1)) == 0) a.inv_counts[i] = 1.0f;
-        if (ln.col < a.dim) store_row<TO, VE>(static_cast<TO*>(a.out) + i * a.out_ld + ln.col, acc, a.scale);
+#pragma unroll
+        for (int t = 0; t < Packs; ++t) {
+            const int col = ln.col + t * 32 * VE;
+            if (col >= a.dim) continue;
+            float2 acc[H] = {};
+            if (row[u] >= 0) {
+                unpack(p[u][t], acc);
+#pragma unroll
+                for (int k = 0; k < H; ++k) acc[k] = mul2_rn(acc[k], make_float2(f[u], f[u]));
+            }
+            store_row<TO, VE>(static_cast<TO*>(a.out) + i * a.out_ld + col, acc, a.scale);
+        }
     }
 }
 
@@ -976,25 +977,25 @@ unsigned grid_of(int64_t warps) {
 // Launches the kernels of the sums; `b` and `so` are the forward and the backward call's.
 template <class T, class TO, int VE, bool Dot, class Entries>
 void launch_sum(SumArgs& a, const Entries& entries, const BagSegments& bags, const SortArgs& so, cudaStream_t s) {
-    constexpr bool forward = std::is_same_v<Entries, TokenEntries>, wide = VE * sizeof(T) == 16;
-    const Tiling narrow(a.dim, VE, 1), t(a.dim, VE, wide ? kMostPacks : 1);
+    constexpr bool forward = std::is_same_v<Entries, TokenEntries>;
+    // several vectors a lane for the widest accesses, and for single elements, of which rows have
+    // the most (in between tiles stay narrow: fewer kernels, for widths that are seldom)
+    constexpr bool several = VE * sizeof(T) == 16 || VE == 1;
+    const Tiling narrow(a.dim, VE, 1), t(a.dim, VE, several ? kMostPacks : 1);
     a.lanes_log2 = t.lanes_log2;
     a.tiles = t.tiles;
     a.piece_tiles = narrow.tiles;
     if (a.n_segments == 0) return;
-    if constexpr (forward) {
-        if (!bags.offsets) {
-            a.tiles = narrow.tiles;
-            const int64_t each = (int64_t)kLookupRows * (32 >> a.lanes_log2);
-            lookup_kernel<T, TO, VE><<<grid_of((a.n_segments + each - 1) / each * a.tiles), kSegmentThreads, 0, s>>>(a, entries);
-            HANNS_CUDA_OK(cudaGetLastError());
-            return;
-        }
-    }
     auto launch = [&](auto packs) {
         constexpr int Packs = decltype(packs)::value;
         if constexpr (forward) {
-            bags_kernel<T, TO, VE, Packs><<<grid_of(a.n_segments * a.tiles), kSegmentThreads, 0, s>>>(a, entries, bags);
+            if (bags.offsets) {
+                bags_kernel<T, TO, VE, Packs><<<grid_of(a.n_segments * a.tiles), kSegmentThreads, 0, s>>>(a, entries, bags);
+            } else {
+                const int64_t each = (int64_t)(kLookupPacks / Packs) * (32 >> a.lanes_log2);
+                lookup_kernel<T, TO, VE, Packs><<<grid_of((a.n_segments + each - 1) / each * a.tiles), kSegmentThreads, 0, s>>>(a,
+                                                                                                                              entries);
+            }
         } else {
             const int64_t warps = so.most_runs * a.tiles + (a.n_segments + 31) / 32;
             runs_kernel<T, TO, VE, Packs, Dot><<<grid_of(warps), kSegmentThreads, 0, s>>>(a, entries, so.runs, so.n_runs, so.most_runs,
@@ -1002,7 +1003,7 @@ void launch_sum(SumArgs& a, const Entries& entries, const BagSegments& bags, con
         }
         HANNS_CUDA_OK(cudaGetLastError());
     };
-    if constexpr (wide) {
+    if constexpr (several) {
         switch (t.packs) {
             case 1: launch(std::integral_constant<int, 1>()); break;
             case 2: launch(std::integral_constant<int, 2>()); break;
@@ -1012,6 +1013,7 @@ void launch_sum(SumArgs& a, const Entries& entries, const BagSegments& bags, con
     } else {
         launch(std::integral_constant<int, 1>());
     }
+    if (forward && !bags.offsets) return;
     if (a.n_entries <= kLimit) return;
     const int64_t most = (a.lists.most_singles + a.lists.most_parts) * a.piece_tiles;
     pieces_kernel<T, TO, VE, Dot><<<(unsigned)std::min<int64_t>(grid_of(most), 16 * 148), kSegmentThreads, 0, s>>>(a, entries);
