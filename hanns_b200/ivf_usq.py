@@ -273,8 +273,8 @@ class IvfUsqIndex:
         return ids, dists
 
     def _check_vectors(self, t, what: str):
-        if not t.is_cuda or t.device.index != self.device:
-            raise ValueError(f"{what} must be on cuda:{self.device}, not {t.device}")
+        if not getattr(t, "is_cuda", False) or t.device.index != self.device:
+            raise ValueError(f"{what} must be a tensor on cuda:{self.device}")
         if t.shape[-1] != self.config.dim:
             raise ValueError("query dimension mismatch")
 

@@ -677,6 +677,120 @@ def test_captured_calls_replay_on_new_inputs():
             assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def capture(step):
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    return graph, out
+
+
+def test_captures_of_every_launch_rule():
+    """One row on a cluster, a warp a row, a block a row; the sort in one block and in several; a
+    lookup; bags with pieces."""
+    cases = []
+    for n, vocab, top in ((1, 128_000, 3), (9, 700, 3), (9, 1900, 0), (700, 9_000, 0), (700, 9_000, 4)):
+        x = some_logits(n, n, vocab, BF16)
+        t = torch.randint(0, vocab, (n,), generator=gen(1)).cuda()
+        g = torch.randn(n, generator=gen(2)).cuda()
+
+        def probs(x=x, t=t, g=g, top=top):
+            z = x.detach().requires_grad_()
+            r = token_logprobs(z, t, top=top)
+            return r.logprobs.detach(), r.entropy.detach(), r.top_tokens, *torch.autograd.grad(r.logprobs, z, g)
+
+        cases.append((probs, lambda x=x: x.neg_()))
+    for n, bags in ((4096, 3), (9001, 40), (5000, 0)):
+        table = torch.randn(800, 48, generator=gen(n)).cuda()
+        tokens = torch.randint(-1, 800, (n,), generator=gen(3)).cuda()
+        offsets = offsets_of([n // bags] * bags + [n % bags]) if bags else None
+        out_rows = n if offsets is None else offsets.numel() - 1
+        g = torch.randn(out_rows, 48, generator=gen(4)).cuda()
+
+        def bag(table=table, tokens=tokens, offsets=offsets, g=g):
+            leaf = table.detach().requires_grad_()
+            out = embed_bags(leaf, tokens, offsets, mean=offsets is not None)
+            return out.detach(), *torch.autograd.grad(out, leaf, g)
+
+        cases.append((bag, lambda tokens=tokens: tokens.copy_(tokens.flip(0))))
+    for step, change in cases:
+        graph, out = capture(step)
+        for _ in range(2):
+            change()
+            want = [o.clone() for o in step()]
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_calls_from_several_threads():
+    import threading
+    table = torch.randn(3000, 200, generator=gen(0)).to(BF16).cuda()
+    tokens, offsets = random_bags(1, 3000, [300, 2, 0, 9000, 40])
+    x = some_logits(1, 40, 30_011, F32)
+    t = torch.randint(0, 30_011, (40,), generator=gen(1)).cuda()
+
+    def work():
+        leaf, z = table.detach().requires_grad_(), x.detach().requires_grad_()
+        out = embed_bags(leaf, tokens, offsets, mean=True, out_dtype=F32)
+        r = token_logprobs(z, t, top=6)
+        return (out.detach(), *torch.autograd.grad(out, leaf, torch.ones_like(out)), r.logprobs.detach(), r.top_tokens,
+                *torch.autograd.grad(r.entropy, z, torch.ones_like(r.entropy)))
+
+    want = work()
+    torch.cuda.synchronize()
+    wrong = []
+
+    def many():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(15):
+                got = work()
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                    wrong.append(1)
+
+    threads = [threading.Thread(target=many) for _ in range(3)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not wrong
+
+
+def test_second_derivatives_are_refused():
+    table = torch.randn(5, 8).cuda().requires_grad_()
+    out = embed_bags(table, torch.tensor([1, 2]).cuda())
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(out.sum(), table, create_graph=True)
+    x = torch.randn(2, 9).cuda().requires_grad_()
+    r = token_logprobs(x, torch.tensor([1, 2]).cuda())
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(r.logprobs.sum(), x, create_graph=True)
+
+
+def test_broadcast_inputs_get_the_sum_of_their_gradients():
+    """One row for the whole table, one weight for all positions, one row of logits for all tokens."""
+    tokens, offsets = random_bags(1, 6, [40, 3, 0, 70], bad=0.0)
+    row = torch.randint(-3, 4, (1, 16), generator=gen(0)).float().cuda().requires_grad_()
+    one = torch.full((1,), 2.0).cuda().requires_grad_()
+    g = torch.randint(-2, 3, (4, 16), generator=gen(1)).float().cuda()
+    d_row, d_one = torch.autograd.grad(embed_bags(row.expand(6, 16), tokens, offsets, one.expand(113)), [row, one], g)
+    lengths = (offsets[1:] - offsets[:-1]).float()
+    assert torch.equal(d_row[0], (g * lengths[:, None]).sum(0) * 2.0)
+    assert d_one[0] == (g * lengths[:, None] * row.detach()).sum()
+    x = some_logits(3, 1, 300, F32).requires_grad_()
+    t = torch.randint(0, 300, (50,), generator=gen(2)).cuda()
+    d, = torch.autograd.grad(token_logprobs(x.expand(50, 300), t).logprobs.sum(), x)
+    want = torch.bincount(t, minlength=300).double() - 50 * torch.softmax(x.detach().double(), 1)
+    # fifty gradients, each within its own roundings, and their sum
+    close(d, want.cpu(), 50 * ((8 * seq_of(300) + 96) * U + 50 * U) * torch.ones(1), "d")
+
+
 @pytest.fixture(scope="module")
 def small_index():
     from hanns_b200 import METRIC_IP, IvfUsqConfig, IvfUsqIndex
@@ -713,6 +827,20 @@ def test_tokens_to_search_to_next_token(small_index, stream):
     check_near(x, given, ids, dist, values, 0.3, 2.0, 1.0, 6)
 
 
+def test_more_probes_than_lists_and_no_rows(small_index):
+    from hanns_b200 import SearchRequest
+    table = torch.randn(50, 64, generator=gen(0)).cuda()
+    tokens, offsets = random_bags(1, 50, [3, 4])
+    a = small_index.search_tokens(table, tokens, offsets, SearchRequest(top_k=4, nprobe=16))
+    b = small_index.search_tokens(table, tokens, offsets, SearchRequest(top_k=4, nprobe=1000))
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    none = torch.zeros(0, dtype=torch.long).cuda()
+    ids, dist = small_index.search_tokens(table, none, none.new_zeros(1), SearchRequest(top_k=4))
+    assert ids.shape == dist.shape == (0, 4)
+    r = small_index.token_logprobs(torch.zeros(0, 64).cuda(), torch.zeros(0, 9).cuda(), none, tokens, SearchRequest(top_k=4), top=2)
+    assert r.logprobs.shape == (0,) and r.top_tokens.shape == (0, 2)
+
+
 def test_index_methods_refuse(small_index):
     from hanns_b200 import SearchRequest
     req = SearchRequest(top_k=3)
@@ -720,6 +848,7 @@ def test_index_methods_refuse(small_index):
     off = torch.tensor([0, 3]).cuda()
     for bad in (lambda: small_index.search_tokens(torch.zeros(5, 63).cuda(), t, off, req),
                 lambda: small_index.search_tokens(torch.zeros(5, 64), t, off, req),
+                lambda: small_index.search_tokens(np.zeros((5, 64), np.float32), t, off, req),
                 lambda: small_index.search_tokens(torch.zeros(5, 64).cuda(), t, None, req),
                 lambda: small_index.token_logprobs(torch.zeros(3, 63).cuda(), torch.zeros(3, 9).cuda(), t, t, req),
                 lambda: small_index.token_logprobs(torch.zeros(2, 64).cuda(), torch.zeros(3, 9).cuda(), t, t, req)):
