@@ -367,6 +367,7 @@ __device__ __forceinline__ void sum_segment(const SumArgs& a, const Lanes& ln, B
 // 16: 21 + 30.
 template <class T, class TO, int VE, int Packs>
 __global__ void __launch_bounds__(kSegmentThreads, blocks_of_sm(Packs, VE, true)) bags_kernel(SumArgs a, TokenEntries entries, BagSegments bags) {
+    wait_for_previous();
     __shared__ Batch batch[kSegmentThreads / 32];
     const uint32_t w = blockIdx.x * (kSegmentThreads / 32) + (threadIdx.x >> 5);
     const uint32_t seg = w / (uint32_t)a.tiles, tile = w - seg * (uint32_t)a.tiles;
@@ -387,6 +388,7 @@ __global__ void __launch_bounds__(kSegmentThreads, blocks_of_sm(Packs, VE, true)
 template <class T, class TO, int VE, int Packs, bool Dot>
 __global__ void __launch_bounds__(kSegmentThreads, blocks_of_sm(Packs, VE, false))
     runs_kernel(SumArgs a, SortedEntries entries, const Run* runs, const int32_t* n_runs, int64_t most_runs, const uint32_t* touched) {
+    wait_for_previous();
     __shared__ Batch batch[kSegmentThreads / 32];
     const int64_t w = (int64_t)blockIdx.x * (kSegmentThreads / 32) + (threadIdx.x >> 5);
     if (w < most_runs * a.tiles) {
@@ -417,6 +419,7 @@ __global__ void __launch_bounds__(kSegmentThreads, blocks_of_sm(Packs, VE, false
 // what counts.  The segment's last warp to arrive adds the pieces, in order.
 template <class T, class TO, int VE, bool Dot, class Entries>
 __global__ void __launch_bounds__(kSegmentThreads, Dot ? 12 : 14) pieces_kernel(SumArgs a, Entries entries) {
+    wait_for_previous();
     constexpr int Packs = 1;
     __shared__ Batch batch[kSegmentThreads / 32];
     const PieceLists& l = a.lists;
@@ -493,6 +496,7 @@ __global__ void __launch_bounds__(kSegmentThreads, Dot ? 12 : 14) pieces_kernel(
 // Bound by memory: 16,384 rows of 768 bf16 take 8.3 us (50 MB).
 template <class T, class TO, int VE, int Packs>
 __global__ void __launch_bounds__(kSegmentThreads) lookup_kernel(SumArgs a, TokenEntries entries) {
+    wait_for_previous();
     constexpr int kRows = kLookupPacks / Packs, H = (VE + 1) / 2;
     const uint32_t w = blockIdx.x * (kSegmentThreads / 32) + (threadIdx.x >> 5);
     const uint32_t batch = w / (uint32_t)a.tiles, tile = w - batch * (uint32_t)a.tiles;
@@ -619,6 +623,7 @@ __device__ __forceinline__ void clear_runs(const SortArgs& a) {  // every thread
 
 template <bool First>
 __global__ void __launch_bounds__(kThreads) sort_count_kernel(SortArgs a) {
+    wait_for_previous();
     __shared__ int32_t count[kMaxBins];
     __shared__ int32_t bag[First ? kSortTile : 1], warp_max[kWarps];
     for (int b = threadIdx.x; b < a.bins; b += kThreads) count[b] = 0;
@@ -658,6 +663,7 @@ __global__ void __launch_bounds__(kThreads) sort_count_kernel(SortArgs a) {
 
 // One warp per digit: its counts become the number of its keys in earlier tiles.
 __global__ void __launch_bounds__(kThreads) sort_scan_kernel(SortArgs a) {
+    wait_for_previous();
     const int bin = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (bin >= a.bins) return;
     int32_t* h = a.hist + (int64_t)bin * a.tiles;
@@ -679,6 +685,7 @@ __global__ void __launch_bounds__(kThreads) sort_scan_kernel(SortArgs a) {
 
 template <bool First, bool Last>
 __global__ void __launch_bounds__(kThreads) sort_move_kernel(SortArgs a) {
+    wait_for_previous();
     __shared__ int32_t seen[kWarps][kMaxBins];  // a warp's keys per digit, then its first place
     __shared__ int32_t warp_sum[kWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -747,6 +754,7 @@ __global__ void __launch_bounds__(kThreads) sort_move_kernel(SortArgs a) {
 
 // Lists each token's run; the thread at its first entry looks for its end, in steps that double.
 __global__ void __launch_bounds__(kThreads) sort_runs_kernel(SortArgs a, const uint32_t* key) {
+    wait_for_previous();
     const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
     uint32_t k = (uint32_t)a.rows;
     if (i < a.n) k = key[i];
@@ -780,6 +788,7 @@ constexpr int kSmallSort = kSmallThreads * kSmallItems, kSmallBits = 8;
 constexpr int64_t kSmallRows = 1 << 20;  // bit maps that one block clears quickly
 
 __global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(SortArgs a, int passes) {
+    wait_for_previous();
     __shared__ uint32_t s_key[kSmallSort];
     __shared__ uint16_t s_pos[kSmallSort];
     __shared__ uint16_t seen[kSmallWarps][1 << kSmallBits];  // a warp's keys per digit, then its first place
@@ -894,6 +903,7 @@ __global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(SortArgs a, i
 
 // dw_j: the column tiles' inner products in order, times scale / c_bag; 0 where j does not count.
 __global__ void __launch_bounds__(kThreads) weights_grad_kernel(const float* dot, int tiles, int piece_tiles, SortArgs a, float* d_weights) {
+    wait_for_previous();
     const int64_t j = (int64_t)blockIdx.x * kThreads + threadIdx.x;
     if (j >= a.n) return;
     const int32_t b = a.bag[j];
@@ -996,15 +1006,15 @@ void launch_sum(SumArgs& a, const Entries& entries, const BagSegments& bags, con
         constexpr int Packs = decltype(packs)::value;
         if constexpr (forward) {
             if (bags.offsets) {
-                bags_kernel<T, TO, VE, Packs><<<grid_of(a.n_segments * a.tiles), kSegmentThreads, 0, s>>>(a, entries, bags);
+                launch_early(bags_kernel<T, TO, VE, Packs>, grid_of(a.n_segments * a.tiles), kSegmentThreads, 0, s, a, entries, bags);
             } else {
                 const int64_t each = (int64_t)(kLookupPacks / Packs) * (32 >> a.lanes_log2);
-                lookup_kernel<T, TO, VE, Packs><<<grid_of((a.n_segments + each - 1) / each * a.tiles), kSegmentThreads, 0, s>>>(a,
+                launch_early(lookup_kernel<T, TO, VE, Packs>, grid_of((a.n_segments + each - 1) / each * a.tiles), kSegmentThreads, 0, s, a,
                                                                                                                               entries);
             }
         } else {
             const int64_t warps = so.most_runs * a.tiles + (a.n_segments + 31) / 32;
-            runs_kernel<T, TO, VE, Packs, Dot><<<grid_of(warps), kSegmentThreads, 0, s>>>(a, entries, so.runs, so.n_runs, so.most_runs,
+            launch_early(runs_kernel<T, TO, VE, Packs, Dot>, grid_of(warps), kSegmentThreads, 0, s, a, entries, so.runs, so.n_runs, so.most_runs,
                                                                                           so.touched);
         }
         HANNS_CUDA_OK(cudaGetLastError());
@@ -1022,7 +1032,7 @@ void launch_sum(SumArgs& a, const Entries& entries, const BagSegments& bags, con
     if (forward && !bags.offsets) return;
     if (a.n_entries <= kLimit) return;
     const int64_t most = (a.lists.most_singles + a.lists.most_parts) * a.piece_tiles;
-    pieces_kernel<T, TO, VE, Dot><<<(unsigned)std::min<int64_t>(grid_of(most), 16 * 148), kSegmentThreads, 0, s>>>(a, entries);
+    launch_early(pieces_kernel<T, TO, VE, Dot, Entries>, (unsigned)std::min<int64_t>(grid_of(most), 16 * 148), kSegmentThreads, 0, s, a, entries);
     HANNS_CUDA_OK(cudaGetLastError());
 }
 
@@ -1094,10 +1104,10 @@ SortPlan sort_plan(int64_t rows, int64_t n) {
 
 template <bool First>
 void sort_pass(const SortArgs& a, bool last, cudaStream_t s) {
-    sort_count_kernel<First><<<a.tiles, kThreads, 0, s>>>(a);
-    sort_scan_kernel<<<(a.bins + kWarps - 1) / kWarps, kThreads, 0, s>>>(a);
-    if (last) sort_move_kernel<First, true><<<a.tiles, kThreads, 0, s>>>(a);
-    else sort_move_kernel<First, false><<<a.tiles, kThreads, 0, s>>>(a);
+    launch_early(sort_count_kernel<First>, a.tiles, kThreads, 0, s, a);
+    launch_early(sort_scan_kernel, (a.bins + kWarps - 1) / kWarps, kThreads, 0, s, a);
+    if (last) launch_early(sort_move_kernel<First, true>, a.tiles, kThreads, 0, s, a);
+    else launch_early(sort_move_kernel<First, false>, a.tiles, kThreads, 0, s, a);
     HANNS_CUDA_OK(cudaGetLastError());
 }
 
@@ -1227,7 +1237,7 @@ extern "C" int32_t hanns_gpu_embed_bags_grad_device(const hanns_embed_bags_t* b,
             while (b->rows >> (passes * kSmallBits)) ++passes;  // keys 0 .. rows
             so.pos_out = gs.pos[0];
             position = so.pos_out;
-            sort_small_kernel<<<1, kSmallThreads, 0, s>>>(so, passes);
+            launch_early(sort_small_kernel, 1, kSmallThreads, 0, s, so, passes);
             HANNS_CUDA_OK(cudaGetLastError());
         } else {
             for (int p = 0; p < sp.passes; ++p) {
@@ -1241,7 +1251,7 @@ extern "C" int32_t hanns_gpu_embed_bags_grad_device(const hanns_embed_bags_t* b,
             }
             sorted = gs.key[sp.passes & 1];
             position = gs.pos[sp.passes & 1];
-            sort_runs_kernel<<<(unsigned)(((int64_t)n + kThreads - 1) / kThreads), kThreads, 0, s>>>(so, sorted);
+            launch_early(sort_runs_kernel, (unsigned)(((int64_t)n + kThreads - 1) / kThreads), kThreads, 0, s, so, sorted);
             HANNS_CUDA_OK(cudaGetLastError());
         }
         SumArgs& a = gs.sum;
@@ -1256,7 +1266,7 @@ extern "C" int32_t hanns_gpu_embed_bags_grad_device(const hanns_embed_bags_t* b,
         a.dot_base = b->table;
         a.dot_ld = b->ld;
         sum_runs<true>(b->out_dtype, b->dtype, a, entries, so, s);
-        weights_grad_kernel<<<(unsigned)(((int64_t)n + kThreads - 1) / kThreads), kThreads, 0, s>>>(a.dot, a.tiles, a.piece_tiles, so,
+        launch_early(weights_grad_kernel, (unsigned)(((int64_t)n + kThreads - 1) / kThreads), kThreads, 0, s, a.dot, a.tiles, a.piece_tiles, so,
                                                                                                    d_weights);
         HANNS_CUDA_OK(cudaGetLastError());
     });

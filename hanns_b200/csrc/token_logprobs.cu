@@ -479,6 +479,7 @@ struct Columns {
 // (with 5 alternatives: 93 -> 107 us).
 template <class T, bool Top>
 __global__ void __launch_bounds__(kMaxThreads, 8) logprobs_kernel(ProbArgs a, int64_t n) {
+    wait_for_previous();
     constexpr int VE = RowView<T>::VE;
     __shared__ Shared sh;
     cg::cluster_group cluster = cg::this_cluster();
@@ -679,6 +680,7 @@ __global__ void __launch_bounds__(kMaxThreads, 8) logprobs_kernel(ProbArgs a, in
 // registers, U a lane, and goes on to another.
 template <class T, bool Top, int U>
 __global__ void __launch_bounds__(kMaxThreads, U > kUnroll ? 6 : 8) logprobs_rows_kernel(ProbArgs a, int64_t n) {
+    wait_for_previous();
     constexpr int VE = RowView<T>::VE, kWarps = kMaxThreads / 32, kRowVectors = 32 * U;
     __shared__ uint64_t buf[kWarps][Top ? kRowVectors : 1], elem[kWarps][Top ? kMaxTop * 8 : 1], top_keys[kWarps][kMaxTop];
     __shared__ int count[kWarps];
@@ -801,6 +803,7 @@ __device__ __forceinline__ void dense_vector(const RowGrad& g, const Pack<float,
 // Bound by memory: 4096 x 128,000 bf16 take 317 us, 6.6 TB/s.
 template <class T, bool Wide>
 __global__ void __launch_bounds__(kGradThreads, 12) logprobs_grad_kernel(GradArgs a) {
+    wait_for_previous();
     constexpr int VE = RowView<T>::VE;
     const int64_t r = blockIdx.x / (unsigned)a.blocks_per_row;
     const int part = (int)(blockIdx.x - r * a.blocks_per_row);
@@ -940,6 +943,7 @@ __device__ __forceinline__ void block_sums(double (&v)[N], double* red) {
 // the alternatives are ordered by sums of two sources, which f32 would tie or swap.
 template <class T>
 __global__ void __launch_bounds__(kMaxThreads) neighbours_kernel(NearArgs a) {
+    wait_for_previous();
     // candidates (log probability, token), neighbours (weight; token, -1 where one does not count)
     extern __shared__ double space[];
     double* cp = space;
@@ -1088,9 +1092,8 @@ void launch_probs(const hanns_token_logprobs_t* t, const ProbArgs& a, cudaStream
     if (vectors <= 32 * 2 * kUnroll) {
         constexpr int warps = kMaxThreads / 32;
         const unsigned blocks = (unsigned)std::min<int64_t>((t->n + warps - 1) / warps, 8 * sm_count());
-        if (vectors <= 32 * kUnroll) logprobs_rows_kernel<T, Top, kUnroll><<<blocks, kMaxThreads, 0, s>>>(a, t->n);
-        else logprobs_rows_kernel<T, Top, 2 * kUnroll><<<blocks, kMaxThreads, 0, s>>>(a, t->n);
-        HANNS_CUDA_OK(cudaGetLastError());
+        if (vectors <= 32 * kUnroll) launch_early(logprobs_rows_kernel<T, Top, kUnroll>, blocks, kMaxThreads, 0, s, a, t->n);
+        else launch_early(logprobs_rows_kernel<T, Top, 2 * kUnroll>, blocks, kMaxThreads, 0, s, a, t->n);
         return;
     }
     // A cluster's blocks share a row when the rows alone are few for the SMs, as long as each block
@@ -1105,11 +1108,13 @@ void launch_probs(const hanns_token_logprobs_t* t, const ProbArgs& a, cudaStream
     cfg.gridDim = dim3((unsigned)(Top || parts > 1 ? t->n * parts : std::min<int64_t>(t->n, 8 * sm_count())));
     cfg.blockDim = dim3((unsigned)threads);
     cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim = {(unsigned)parts, 1, 1};
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim = {(unsigned)parts, 1, 1};
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     HANNS_CUDA_OK(cudaLaunchKernelEx(&cfg, logprobs_kernel<T, Top>, a, t->n));
 }
 
@@ -1127,8 +1132,8 @@ void launch_grad(const hanns_token_logprobs_t* t, GradArgs a, cudaStream_t s) {
     // wide stores where each output row starts as its logits do within 16 bytes
     const bool wide = ((uintptr_t)a.logits - (uintptr_t)a.out) % 16 == 0 && ((a.ld - a.out_ld) * (int64_t)sizeof(T)) % 16 == 0;
     const unsigned grid = (unsigned)(t->n * a.blocks_per_row);
-    if (wide) logprobs_grad_kernel<T, true><<<grid, kGradThreads, 0, s>>>(a);
-    else logprobs_grad_kernel<T, false><<<grid, kGradThreads, 0, s>>>(a);
+    if (wide) launch_early(logprobs_grad_kernel<T, true>, grid, kGradThreads, 0, s, a);
+    else launch_early(logprobs_grad_kernel<T, false>, grid, kGradThreads, 0, s, a);
     HANNS_CUDA_OK(cudaGetLastError());
 }
 
@@ -1234,9 +1239,9 @@ extern "C" int32_t hanns_gpu_neighbour_logprobs_device(const hanns_token_logprob
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         const unsigned threads = k <= 32 ? 32 : k <= 64 ? 64 : kMaxThreads, n = (unsigned)t->n;
         const size_t shared = (2 * (size_t)k + a.top) * sizeof(double) + (2 * (size_t)k + a.top) * sizeof(int32_t);
-        if (t->dtype == HANNS_DTYPE_F32) neighbours_kernel<float><<<n, threads, shared, s>>>(a);
-        else if (t->dtype == HANNS_DTYPE_F16) neighbours_kernel<__half><<<n, threads, shared, s>>>(a);
-        else neighbours_kernel<__nv_bfloat16><<<n, threads, shared, s>>>(a);
+        if (t->dtype == HANNS_DTYPE_F32) launch_early(neighbours_kernel<float>, n, threads, shared, s, a);
+        else if (t->dtype == HANNS_DTYPE_F16) launch_early(neighbours_kernel<__half>, n, threads, shared, s, a);
+        else launch_early(neighbours_kernel<__nv_bfloat16>, n, threads, shared, s, a);
         HANNS_CUDA_OK(cudaGetLastError());
     });
 }
