@@ -40,7 +40,9 @@ constexpr int kDots = 8;              // inner products that are reduced togethe
 // that its registers are kept to (more spill, fewer leave the memory idle).
 constexpr int kMostPacks = 4;
 __host__ __device__ constexpr int rows_ahead(int packs) { return packs == 1 ? 8 : packs == 2 ? 3 : 2; }
-constexpr int blocks_of_sm(int packs, int ve, bool forward) { return packs == 1 ? 14 : ve == 1 ? 16 : forward ? (ve == 8 ? 16 : 18) : ve == 8 ? 10 : 14; }
+constexpr int blocks_of_sm(int packs, int ve, bool forward) {
+    return packs == 1 ? 14 : ve == 1 ? 16 : forward ? (ve == 8 ? 16 : 18) : ve == 8 ? 10 : 14;
+}
 constexpr int kLookupPacks = 8;       // vectors of a lane in a lookup
 constexpr int kMaxBinBits = 9, kMaxBins = 1 << kMaxBinBits;
 constexpr int kSortItems = 4, kSortTile = kThreads * kSortItems;
@@ -213,9 +215,10 @@ struct Batch {
 // Entries q, q + groups, ... of a batch of n, N per group (all there when Full).  step[t]: column of
 // vector t; vectors behind the row's end are the first one's again.
 template <class T, int VE, int Packs, bool Dot, int N, bool Full>
-__device__ __forceinline__ void add_rows(const SumArgs& a, const Lanes& ln, const Batch& bt, const char* base, const int (&step)[Packs],
-                                         int q, int n, float2 (&acc)[Packs][(VE + 1) / 2], const float2 (&e)[Packs][(VE + 1) / 2],
-                                         float* dot) {
+__device__ __forceinline__ void add_rows(const SumArgs& a, const Lanes& ln, const Batch& bt, const char* base,
+                                         const int (&step)[Packs], int q, int n,
+                                         float2 (&acc)[Packs][(VE + 1) / 2],
+                                         const float2 (&e)[Packs][(VE + 1) / 2], float* dot) {
     constexpr int H = (VE + 1) / 2;
     Pack<T, VE> p[N][Packs];
     float d[kDots] = {};
@@ -267,8 +270,9 @@ __device__ __forceinline__ void add_rows(const SumArgs& a, const Lanes& ln, cons
 // behind the last column are another's and are not stored).  Returns the number of counted
 // entries.
 template <class T, class TE, int VE, int Packs, bool Dot, class Entries>
-__device__ __forceinline__ int sum_entries(const SumArgs& a, const Lanes& ln, Batch& bt, const Entries& entries, int64_t lo, int64_t hi,
-                                           const TE* dot_row, float* dot, float2 (&acc)[Packs][(VE + 1) / 2]) {
+__device__ __forceinline__ int sum_entries(const SumArgs& a, const Lanes& ln, Batch& bt, const Entries& entries,
+                                           int64_t lo, int64_t hi, const TE* dot_row, float* dot,
+                                           float2 (&acc)[Packs][(VE + 1) / 2]) {
     constexpr int H = (VE + 1) / 2, N = rows_ahead(Packs), Tail = (N + 1) / 2;
     static_assert(N <= kDots, "reduce_dots takes a round's products");
     int step[Packs];
@@ -324,8 +328,8 @@ __device__ __forceinline__ int sum_entries(const SumArgs& a, const Lanes& ln, Ba
 
 // Stores a lane's vectors of a row.
 template <class TO, int VE, int Packs>
-__device__ __forceinline__ void store_sums(const SumArgs& a, const Lanes& ln, TO* row, const float2 (&acc)[Packs][(VE + 1) / 2],
-                                           float factor) {
+__device__ __forceinline__ void store_sums(const SumArgs& a, const Lanes& ln, TO* row,
+                                           const float2 (&acc)[Packs][(VE + 1) / 2], float factor) {
     if (ln.lane >= ln.count) return;
 #pragma unroll
     for (int t = 0; t < Packs; ++t)
@@ -337,7 +341,7 @@ __device__ __forceinline__ void list_pieces(const SumArgs& a, int lane, int32_t 
     const PieceLists& l = a.lists;
     // the square root: one after the other come a piece's entries and then the pieces
     const int length = max(l.length, (int)sqrtf(1.5f * (float)(hi - lo)));
-    const int n = (hi - lo + length - 1) / length;
+    const int n = (int)(((int64_t)(hi - lo) + length - 1) / length);
     int32_t first = 0;
     if (lane == 0) first = atomicAdd(l.count + (n > 1), n);
     first = __shfl_sync(0xffffffffu, first, 0);
@@ -345,18 +349,21 @@ __device__ __forceinline__ void list_pieces(const SumArgs& a, int lane, int32_t 
     const int64_t room = n > 1 ? l.most_parts : l.most_singles;
     if (first < 0) return;
     for (int i = lane; i < n && first + (int64_t)i < room; i += 32)
-        to[first + (int64_t)i] = Piece{seg, lo + i * length, min(hi, lo + (i + 1) * length), i, first, n, {0, 0}};
+        to[first + (int64_t)i] = Piece{seg,   lo + i * length, (int32_t)min((int64_t)hi, lo + (i + 1) * (int64_t)length),
+                                       i,     first,           n,
+                                       {0, 0}};
     if (n > 1 && first < room)
         for (int t = lane; t < a.piece_tiles; t += 32) l.arrived[(int64_t)first * a.piece_tiles + t] = 0;
 }
 
 // A segment's row (of not more than kLimit entries) by one warp and column tile.
 template <class T, class TO, int VE, int Packs, bool Dot, class Entries>
-__device__ __forceinline__ void sum_segment(const SumArgs& a, const Lanes& ln, Batch& bt, const Entries& entries, int64_t seg, int64_t lo,
-                                            int64_t hi, int tile) {
+__device__ __forceinline__ void sum_segment(const SumArgs& a, const Lanes& ln, Batch& bt, const Entries& entries,
+                                            int64_t seg, int64_t lo, int64_t hi, int tile) {
     float2 acc[Packs][(VE + 1) / 2];
-    const int count = sum_entries<T, TO, VE, Packs, Dot>(a, ln, bt, entries, lo, hi, static_cast<const TO*>(a.dot_base) + seg * a.dot_ld,
-                                                         a.dot + (int64_t)tile * a.n_entries, acc);
+    const TO* dot_row = static_cast<const TO*>(a.dot_base) + seg * a.dot_ld;
+    float* dot = a.dot + (int64_t)tile * a.n_entries;
+    const int count = sum_entries<T, TO, VE, Packs, Dot>(a, ln, bt, entries, lo, hi, dot_row, dot, acc);
     const float f = finish_factor(a, seg, count, tile == 0 && ln.lane == 0);
     store_sums<TO, VE, Packs>(a, ln, static_cast<TO*>(a.out) + seg * a.out_ld, acc, f);
 }
@@ -366,7 +373,8 @@ __device__ __forceinline__ void sum_segment(const SumArgs& a, const Lanes& ln, B
 // of vectors) take 25 us, 9 TB/s.  Longest bag here 32: 25 + 15 us with the pieces, 64: 37 + 14,
 // 16: 21 + 30.
 template <class T, class TO, int VE, int Packs>
-__global__ void __launch_bounds__(kSegmentThreads, blocks_of_sm(Packs, VE, true)) bags_kernel(SumArgs a, TokenEntries entries, BagSegments bags) {
+__global__ void __launch_bounds__(kSegmentThreads, blocks_of_sm(Packs, VE, true))
+    bags_kernel(SumArgs a, TokenEntries entries, BagSegments bags) {
     wait_for_previous();
     __shared__ Batch batch[kSegmentThreads / 32];
     const uint32_t w = blockIdx.x * (kSegmentThreads / 32) + (threadIdx.x >> 5);
@@ -387,7 +395,8 @@ __global__ void __launch_bounds__(kSegmentThreads, blocks_of_sm(Packs, VE, true)
 // pieces of tokens that occur more than 32 times (59 % of the positions).
 template <class T, class TO, int VE, int Packs, bool Dot>
 __global__ void __launch_bounds__(kSegmentThreads, blocks_of_sm(Packs, VE, false))
-    runs_kernel(SumArgs a, SortedEntries entries, const Run* runs, const int32_t* n_runs, int64_t most_runs, const uint32_t* touched) {
+    runs_kernel(SumArgs a, SortedEntries entries, const Run* runs, const int32_t* n_runs, int64_t most_runs,
+                const uint32_t* touched) {
     wait_for_previous();
     __shared__ Batch batch[kSegmentThreads / 32];
     const int64_t w = (int64_t)blockIdx.x * (kSegmentThreads / 32) + (threadIdx.x >> 5);
@@ -423,11 +432,13 @@ __global__ void __launch_bounds__(kSegmentThreads, Dot ? 12 : 14) pieces_kernel(
     constexpr int Packs = 1;
     __shared__ Batch batch[kSegmentThreads / 32];
     const PieceLists& l = a.lists;
-    const int64_t n_parts = min((int64_t)max(l.count[1], 0), l.most_parts), n_singles = min((int64_t)max(l.count[0], 0), l.most_singles);
+    const int64_t n_parts = min((int64_t)max(l.count[1], 0), l.most_parts);
+    const int64_t n_singles = min((int64_t)max(l.count[0], 0), l.most_singles);
     const int64_t items = (n_parts + n_singles) * a.piece_tiles;
     const int width = (a.piece_tiles << a.lanes_log2) * VE;
     constexpr int of_block = kSegmentThreads / 32;
-    for (int64_t item = (int64_t)blockIdx.x * of_block + (threadIdx.x >> 5); item < items; item += (int64_t)gridDim.x * of_block) {
+    for (int64_t item = (int64_t)blockIdx.x * of_block + (threadIdx.x >> 5); item < items;
+         item += (int64_t)gridDim.x * of_block) {
         const int64_t at = item / a.piece_tiles;
         const int tile = (int)(item - at * a.piece_tiles);
         const Lanes ln(a, tile, VE, Packs);
@@ -448,7 +459,8 @@ __global__ void __launch_bounds__(kSegmentThreads, Dot ? 12 : 14) pieces_kernel(
             count = 0;
             const int n = (int)min((int64_t)pc.n, l.most_parts - pc.first);
             if (a.mean) {
-                for (int i = ln.lane; i < n; i += 32) count += __ldcg(l.partial_count + (int64_t)(pc.first + i) * a.piece_tiles + tile);
+                for (int i = ln.lane; i < n; i += 32)
+                    count += __ldcg(l.partial_count + (int64_t)(pc.first + i) * a.piece_tiles + tile);
                 count = __reduce_add_sync(0xffffffffu, count);
             }
 #pragma unroll
@@ -618,7 +630,8 @@ __device__ __forceinline__ void clear_runs(const SortArgs& a) {  // every thread
     const int64_t i0 = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i0 < 2) a.list_counts[i0] = 0;
     if (i0 == 2) *a.n_runs = 0;
-    for (int64_t i = i0; i < (a.rows + 31) / 32; i += (int64_t)gridDim.x * blockDim.x) a.touched[i] = a.lengthy[i] = 0;
+    for (int64_t i = i0; i < (a.rows + 31) / 32; i += (int64_t)gridDim.x * blockDim.x)
+        a.touched[i] = a.lengthy[i] = 0;
 }
 
 template <bool First>
@@ -819,7 +832,8 @@ __global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(SortArgs a, i
     }
     for (int p = 0; p < passes; ++p) {
         const int shift = p * kSmallBits;
-        for (int b = threadIdx.x; b < kSmallWarps << (kSmallBits - 1); b += kSmallThreads) reinterpret_cast<uint32_t*>(&seen[0][0])[b] = 0;
+        uint32_t* words = reinterpret_cast<uint32_t*>(&seen[0][0]);
+        for (int b = threadIdx.x; b < kSmallWarps << (kSmallBits - 1); b += kSmallThreads) words[b] = 0;
         __syncthreads();
         int rank[kSmallItems];
 #pragma unroll
@@ -902,7 +916,8 @@ __global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(SortArgs a, i
 }
 
 // dw_j: the column tiles' inner products in order, times scale / c_bag; 0 where j does not count.
-__global__ void __launch_bounds__(kThreads) weights_grad_kernel(const float* dot, int tiles, int piece_tiles, SortArgs a, float* d_weights) {
+__global__ void __launch_bounds__(kThreads)
+    weights_grad_kernel(const float* dot, int tiles, int piece_tiles, SortArgs a, float* d_weights) {
     wait_for_previous();
     const int64_t j = (int64_t)blockIdx.x * kThreads + threadIdx.x;
     if (j >= a.n) return;
@@ -1006,18 +1021,18 @@ void launch_sum(SumArgs& a, const Entries& entries, const BagSegments& bags, con
         constexpr int Packs = decltype(packs)::value;
         if constexpr (forward) {
             if (bags.offsets) {
-                launch_early(bags_kernel<T, TO, VE, Packs>, grid_of(a.n_segments * a.tiles), kSegmentThreads, 0, s, a, entries, bags);
+                launch_early(bags_kernel<T, TO, VE, Packs>, grid_of(a.n_segments * a.tiles), kSegmentThreads, 0, s, a,
+                             entries, bags);
             } else {
                 const int64_t each = (int64_t)(kLookupPacks / Packs) * (32 >> a.lanes_log2);
-                launch_early(lookup_kernel<T, TO, VE, Packs>, grid_of((a.n_segments + each - 1) / each * a.tiles), kSegmentThreads, 0, s, a,
-                                                                                                                              entries);
+                const unsigned grid = grid_of((a.n_segments + each - 1) / each * a.tiles);
+                launch_early(lookup_kernel<T, TO, VE, Packs>, grid, kSegmentThreads, 0, s, a, entries);
             }
         } else {
             const int64_t warps = so.most_runs * a.tiles + (a.n_segments + 31) / 32;
-            launch_early(runs_kernel<T, TO, VE, Packs, Dot>, grid_of(warps), kSegmentThreads, 0, s, a, entries, so.runs, so.n_runs, so.most_runs,
-                                                                                          so.touched);
+            launch_early(runs_kernel<T, TO, VE, Packs, Dot>, grid_of(warps), kSegmentThreads, 0, s, a, entries, so.runs,
+                         so.n_runs, so.most_runs, so.touched);
         }
-        HANNS_CUDA_OK(cudaGetLastError());
     };
     if constexpr (several) {
         switch (t.packs) {
@@ -1032,15 +1047,16 @@ void launch_sum(SumArgs& a, const Entries& entries, const BagSegments& bags, con
     if (forward && !bags.offsets) return;
     if (a.n_entries <= kLimit) return;
     const int64_t most = (a.lists.most_singles + a.lists.most_parts) * a.piece_tiles;
-    launch_early(pieces_kernel<T, TO, VE, Dot, Entries>, (unsigned)std::min<int64_t>(grid_of(most), 16 * 148), kSegmentThreads, 0, s, a, entries);
-    HANNS_CUDA_OK(cudaGetLastError());
+    const unsigned blocks = (unsigned)std::min<int64_t>(grid_of(most), 16 * 148);
+    launch_early(pieces_kernel<T, TO, VE, Dot, Entries>, blocks, kSegmentThreads, 0, s, a, entries);
 }
 
 // In: type of the summed rows, Out: of the result (and of the rows of the inner products).
 template <class T, class TO, bool Dot, class Entries>
 void sum_segments(SumArgs& a, const Entries& entries, const BagSegments& bags, const SortArgs& so, cudaStream_t s) {
     const Matrix in{a.base, a.ld, sizeof(T)}, out{a.out, a.out_ld, sizeof(TO)};
-    const int ve = Dot ? vector_elems(a.dim, {in, out, Matrix{a.dot_base, a.dot_ld, sizeof(TO)}}) : vector_elems(a.dim, {in, out});
+    const Matrix table = Dot ? Matrix{a.dot_base, a.dot_ld, sizeof(TO)} : out;
+    const int ve = vector_elems(a.dim, {in, out, table});
     constexpr int wide = 16 / sizeof(T);
     if (ve == wide) return launch_sum<T, TO, wide, Dot>(a, entries, bags, so, s);
     if (ve == wide / 2) return launch_sum<T, TO, wide / 2, Dot>(a, entries, bags, so, s);
@@ -1108,7 +1124,6 @@ void sort_pass(const SortArgs& a, bool last, cudaStream_t s) {
     launch_early(sort_scan_kernel, (a.bins + kWarps - 1) / kWarps, kThreads, 0, s, a);
     if (last) launch_early(sort_move_kernel<First, true>, a.tiles, kThreads, 0, s, a);
     else launch_early(sort_move_kernel<First, false>, a.tiles, kThreads, 0, s, a);
-    HANNS_CUDA_OK(cudaGetLastError());
 }
 
 // Workspace of a gradient call, carved alike when it is counted and when it is used.
@@ -1211,7 +1226,8 @@ extern "C" int32_t hanns_gpu_embed_bags_grad_device(const hanns_embed_bags_t* b,
         require(grad || b->n_bags == 0, "embed_bags: null gradient");
         require(b->tokens || b->n_tokens == 0, "embed_bags: null tokens");
         require(!b->mean || b->inv_counts || b->n_bags == 0, "embed_bags: a mean's gradient needs inv_counts");
-        require(!d_weights || (b->table && b->weights), "embed_bags: the weights' gradient needs the table and the weights");
+        require(!d_weights || (b->table && b->weights),
+                "embed_bags: the weights' gradient needs the table and the weights");
         check_workspace((size_t)hanns_gpu_embed_bags_grad_workspace_bytes(b), b->workspace, b->workspace_bytes);
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         const SortPlan sp = sort_plan(b->rows, b->n_tokens);
@@ -1228,6 +1244,7 @@ extern "C" int32_t hanns_gpu_embed_bags_grad_device(const hanns_embed_bags_t* b,
         so.tiles = sp.tiles;
         so.scale = b->scale;
         so.bins = 1 << sp.bits;
+        const unsigned by_position = (unsigned)(((int64_t)n + kThreads - 1) / kThreads);
         const uint32_t *sorted = nullptr, *position = nullptr;
         if (n == 0) {
             HANNS_CUDA_OK(cudaMemsetAsync(so.touched, 0, (b->rows + 31) / 32 * sizeof(uint32_t), s));
@@ -1238,7 +1255,6 @@ extern "C" int32_t hanns_gpu_embed_bags_grad_device(const hanns_embed_bags_t* b,
             so.pos_out = gs.pos[0];
             position = so.pos_out;
             launch_early(sort_small_kernel, 1, kSmallThreads, 0, s, so, passes);
-            HANNS_CUDA_OK(cudaGetLastError());
         } else {
             for (int p = 0; p < sp.passes; ++p) {
                 so.shift = p * sp.bits;
@@ -1251,8 +1267,7 @@ extern "C" int32_t hanns_gpu_embed_bags_grad_device(const hanns_embed_bags_t* b,
             }
             sorted = gs.key[sp.passes & 1];
             position = gs.pos[sp.passes & 1];
-            launch_early(sort_runs_kernel, (unsigned)(((int64_t)n + kThreads - 1) / kThreads), kThreads, 0, s, so, sorted);
-            HANNS_CUDA_OK(cudaGetLastError());
+            launch_early(sort_runs_kernel, by_position, kThreads, 0, s, so, sorted);
         }
         SumArgs& a = gs.sum;
         a.base = grad;
@@ -1266,8 +1281,6 @@ extern "C" int32_t hanns_gpu_embed_bags_grad_device(const hanns_embed_bags_t* b,
         a.dot_base = b->table;
         a.dot_ld = b->ld;
         sum_runs<true>(b->out_dtype, b->dtype, a, entries, so, s);
-        launch_early(weights_grad_kernel, (unsigned)(((int64_t)n + kThreads - 1) / kThreads), kThreads, 0, s, a.dot, a.tiles, a.piece_tiles, so,
-                                                                                                   d_weights);
-        HANNS_CUDA_OK(cudaGetLastError());
+        launch_early(weights_grad_kernel, by_position, kThreads, 0, s, a.dot, a.tiles, a.piece_tiles, so, d_weights);
     });
 }

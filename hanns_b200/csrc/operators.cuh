@@ -50,7 +50,8 @@ __device__ __forceinline__ void wait_for_previous() {
     cudaGridDependencySynchronize();
 }
 template <class... Params, class... Args>
-void launch_early(void (*kernel)(Params...), unsigned grid, unsigned block, size_t shared, cudaStream_t s, Args&&... args) {
+void launch_early(void (*kernel)(Params...), unsigned grid, unsigned block, size_t shared, cudaStream_t s,
+                  Args&&... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(block);

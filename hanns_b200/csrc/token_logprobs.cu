@@ -10,10 +10,11 @@
 // logprobs_kernel reads the logits once: running maximum, sum and weighted sum per thread
 // (rescaled when the maximum grows).  Exponents are in powers of two, y = x c - R with
 // c = log2(e) / T and the reference R = m c as f32 rounds it: any R serves, since the same one
-// is taken off again, and y then has a single rounding.  The alternatives come from a threshold
-// that a first look at the row sets; the few vectors above it go to a buffer in shared memory.
-// A row is one block's, or a cluster's when there are few rows: each block of the cluster then
-// takes a share of the columns and the first one joins them over distributed shared memory.
+// is taken off again, and y then has a single rounding.  For the alternatives each thread keeps
+// the maxima of its two largest rounds of loads; the `top`-th of the threads' maxima bounds the
+// row's `top`-th logit, and the few rounds that reach the bound are read again, from the L2.  A row
+// is one block's, or a cluster's when there are few rows: each block of the cluster then takes a
+// share of the columns and the first one joins them over distributed shared memory.
 //
 // neighbours_kernel mixes in the tokens of a search's neighbours:
 //   w = softmax(-distance / tau),  p_v = (1 - l) q_v + l sum of w_j over neighbours j with token v
@@ -415,8 +416,8 @@ __device__ void select_again(Shared& sh, const RowView<T>& view, int v0, int v1,
 
 // A row's outputs from its maximum, reference and sums.
 template <class Group>
-__device__ __forceinline__ void write_row(const ProbArgs& a, int64_t r, int64_t token, float x_t, float m, float ref, float s,
-                                          float u, bool differences, const uint64_t* best) {
+__device__ __forceinline__ void write_row(const ProbArgs& a, int64_t r, int64_t token, float x_t, float m, float ref,
+                                          float s, float u, bool differences, const uint64_t* best) {
     const bool empty = m == -INFINITY, undefined = !(m < INFINITY);
     // the sum of e^((x - m) / T): the reference is m c but for f32's rounding of it
     const float s_m = differences ? s : s * exp2f(-fmaf(m, a.c, -ref)), log_s = logf(s_m);
@@ -546,7 +547,8 @@ __global__ void __launch_bounds__(kMaxThreads, 8) logprobs_kernel(ProbArgs a, in
             }
             for (uint32_t who = __ballot_sync(0xffffffffu, many); who; who &= who - 1) {
                 const int j0 = b0 + (int)(threadIdx.x & ~31u) + __ffs(who) - 1;
-                for (int j = j0 + (int)(threadIdx.x & 31) * (int)blockDim.x; j < b1; j += 32 * (int)blockDim.x) offer_vector(j);
+                for (int j = j0 + (int)(threadIdx.x & 31) * (int)blockDim.x; j < b1; j += 32 * (int)blockDim.x)
+                    offer_vector(j);
             }
         }
         // the partial vectors at the row's ends
@@ -676,13 +678,14 @@ __global__ void __launch_bounds__(kMaxThreads, 8) logprobs_kernel(ProbArgs a, in
     }
 }
 
-// Short rows (8192 x 1000 bf16: 7.9 us, with 5 alternatives 14.3): a warp takes a row whose vectors (the partial ones among them) fit in its
-// registers, U a lane, and goes on to another.
+// Short rows (8192 x 1000 bf16: 7.9 us, with 5 alternatives 14.3): a warp takes a row whose vectors
+// (the partial ones among them) fit in its registers, U a lane, and goes on to another.
 template <class T, bool Top, int U>
 __global__ void __launch_bounds__(kMaxThreads, U > kUnroll ? 6 : 8) logprobs_rows_kernel(ProbArgs a, int64_t n) {
     wait_for_previous();
     constexpr int VE = RowView<T>::VE, kWarps = kMaxThreads / 32, kRowVectors = 32 * U;
-    __shared__ uint64_t buf[kWarps][Top ? kRowVectors : 1], elem[kWarps][Top ? kMaxTop * 8 : 1], top_keys[kWarps][kMaxTop];
+    __shared__ uint64_t buf[kWarps][Top ? kRowVectors : 1], elem[kWarps][Top ? kMaxTop * 8 : 1];
+    __shared__ uint64_t top_keys[kWarps][kMaxTop];
     __shared__ int count[kWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Choice ch{buf[warp], kRowVectors, elem[warp], top_keys[warp], &count[warp]};
@@ -876,10 +879,12 @@ __global__ void __launch_bounds__(kGradThreads, 12) logprobs_grad_kernel(GradArg
             }
         }
     }
-    const int64_t head = view.skipped() ? min((int64_t)a.vocab, view.first(1)) : 0, tail = head + (int64_t)view.n * VE;
+    const int64_t head = view.skipped() ? min((int64_t)a.vocab, view.first(1)) : 0;
+    const int64_t tail = head + (int64_t)view.n * VE;
     if (part == 0 && threadIdx.x < 2 * VE) {
         const int64_t e = (int)threadIdx.x < VE ? (int64_t)threadIdx.x : tail + threadIdx.x - VE;
-        if ((int)threadIdx.x < VE ? e < head : e < a.vocab) out[e] = from_f32<T>(live ? rg.dense(to_f32(row[e])) : rg.base);
+        if ((int)threadIdx.x < VE ? e < head : e < a.vocab)
+            out[e] = from_f32<T>(live ? rg.dense(to_f32(row[e])) : rg.base);
     }
     // the given token and the alternatives have terms of their own
     if (!live) return;
@@ -1086,14 +1091,16 @@ constexpr int sm_count() { return 148; }
 
 template <class T, bool Top>
 void launch_probs(const hanns_token_logprobs_t* t, const ProbArgs& a, cudaStream_t s) {
-    const int64_t vectors = (t->vocab + RowView<T>::VE - 1) / RowView<T>::VE + 1;  // one more where a row starts inside a vector
+    // one more where a row starts inside a vector
+    const int64_t vectors = (t->vocab + RowView<T>::VE - 1) / RowView<T>::VE + 1;
     // A warp for a row that fits in its registers, 4 or 8 vectors a lane: 8192 rows of 100 f32 with 5
     // alternatives take 10.5 us (a block each: 36.8), of 2,000 bf16 21.9 us (43.1).
     if (vectors <= 32 * 2 * kUnroll) {
         constexpr int warps = kMaxThreads / 32;
         const unsigned blocks = (unsigned)std::min<int64_t>((t->n + warps - 1) / warps, 8 * sm_count());
-        if (vectors <= 32 * kUnroll) launch_early(logprobs_rows_kernel<T, Top, kUnroll>, blocks, kMaxThreads, 0, s, a, t->n);
-        else launch_early(logprobs_rows_kernel<T, Top, 2 * kUnroll>, blocks, kMaxThreads, 0, s, a, t->n);
+        auto* kernel = vectors <= 32 * kUnroll ? logprobs_rows_kernel<T, Top, kUnroll>
+                                               : logprobs_rows_kernel<T, Top, 2 * kUnroll>;
+        launch_early(kernel, blocks, kMaxThreads, 0, s, a, t->n);
         return;
     }
     // A cluster's blocks share a row when the rows alone are few for the SMs, as long as each block
@@ -1101,7 +1108,8 @@ void launch_probs(const hanns_token_logprobs_t* t, const ProbArgs& a, cudaStream
     // 18.6); 300 rows of 50,257 with alternatives 13.7 us (on two blocks each 15.0).
     int parts = 1;
     const int64_t want = 4 * sm_count();
-    while (parts < kMaxCluster && t->n * parts * 2 <= want && vectors / (parts * 2) >= kMaxThreads * kUnroll) parts *= 2;
+    while (parts < kMaxCluster && t->n * parts * 2 <= want && vectors / (parts * 2) >= kMaxThreads * kUnroll)
+        parts *= 2;
     const int threads = kMaxThreads;
     cudaLaunchConfig_t cfg{};
     // blocks that take several rows: as many as are resident
@@ -1125,16 +1133,17 @@ void launch_grad(const hanns_token_logprobs_t* t, GradArgs a, cudaStream_t s) {
     // rows of 32,000 f32: 21.7 us, one round each 28.1)
     const int64_t round = kGradThreads * kGradUnroll;
     int64_t rounds = kGradRounds;
-    while (rounds > 1 && t->n * ((vectors + rounds * round - 1) / (rounds * round)) < 16 * sm_count()) rounds /= 2;
+    while (rounds > 1 && t->n * ((vectors + rounds * round - 1) / (rounds * round)) < 16 * sm_count())
+        rounds /= 2;
     a.span = (int)(rounds * round);
     a.blocks_per_row = (int)((vectors + a.span - 1) / a.span);
     require(t->n * a.blocks_per_row < 0x7fffffff, "token_logprobs: too many elements for one gradient call");
     // wide stores where each output row starts as its logits do within 16 bytes
-    const bool wide = ((uintptr_t)a.logits - (uintptr_t)a.out) % 16 == 0 && ((a.ld - a.out_ld) * (int64_t)sizeof(T)) % 16 == 0;
+    const bool wide = ((uintptr_t)a.logits - (uintptr_t)a.out) % 16 == 0 &&
+                      ((a.ld - a.out_ld) * (int64_t)sizeof(T)) % 16 == 0;
     const unsigned grid = (unsigned)(t->n * a.blocks_per_row);
     if (wide) launch_early(logprobs_grad_kernel<T, true>, grid, kGradThreads, 0, s, a);
     else launch_early(logprobs_grad_kernel<T, false>, grid, kGradThreads, 0, s, a);
-    HANNS_CUDA_OK(cudaGetLastError());
 }
 
 template <class T>
@@ -1242,6 +1251,5 @@ extern "C" int32_t hanns_gpu_neighbour_logprobs_device(const hanns_token_logprob
         if (t->dtype == HANNS_DTYPE_F32) launch_early(neighbours_kernel<float>, n, threads, shared, s, a);
         else if (t->dtype == HANNS_DTYPE_F16) launch_early(neighbours_kernel<__half>, n, threads, shared, s, a);
         else launch_early(neighbours_kernel<__nv_bfloat16>, n, threads, shared, s, a);
-        HANNS_CUDA_OK(cudaGetLastError());
     });
 }
