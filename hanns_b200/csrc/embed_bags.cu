@@ -94,6 +94,20 @@ struct BagSegments {
         }
         return a;
     }
+    // The same by a whole warp, a 32nd of the range a step.
+    __device__ __forceinline__ int64_t starts_up_to_by_warp(int64_t p) const {
+        const int lane = threadIdx.x & 31;
+        int64_t a = 0, n = n_bags + 1;  // the answer is in [a, a + n]
+        while (n > 0) {
+            const int64_t step = (n + 31) / 32, at = a + lane * step;  // lane's part: [at, at + step)
+            const bool below = at + step - 1 < a + n && offsets[at + step - 1] <= p;
+            const int parts = __popc(__ballot_sync(0xffffffffu, below));
+            a += parts * step;
+            n = parts == 32 ? 0 : min(step - 1, n - parts * step);
+            if (n < 0) n = 0;
+        }
+        return a;
+    }
 };
 // A token's run of entries in the sorted order.
 struct Run {
@@ -589,7 +603,7 @@ __device__ void tile_bags(const BagSegments& bags, int64_t base, int32_t (&bag)[
         __syncthreads();
         return;
     }
-    const int32_t before = (int32_t)bags.starts_up_to(base);
+    const int32_t before = (int32_t)bags.starts_up_to_by_warp(base);
     for (int i = threadIdx.x; i < kSortTile; i += kThreads) bag[i] = before;
     __syncthreads();
     for (int64_t k = before + threadIdx.x; k <= bags.n_bags; k += kThreads) {

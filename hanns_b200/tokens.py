@@ -70,12 +70,13 @@ def _rows(t):
     return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
-def _run(dev, work):
-    """work(stream) with dev current, on dev's current stream."""
-    if torch.cuda.current_device() == dev.index:
-        return work(torch._C._cuda_getCurrentRawStream(dev.index))
+def _run(dev, work, *args):
+    """work(stream, *args) with dev current, on dev's current stream."""
+    index = dev.index
+    if torch.cuda.current_device() == index:
+        return work(torch._C._cuda_getCurrentRawStream(index), *args)
     with torch.cuda.device(dev):
-        return work(torch._C._cuda_getCurrentRawStream(dev.index))
+        return work(torch._C._cuda_getCurrentRawStream(index), *args)
 
 
 def _workspace(nbytes, device, b):
@@ -111,14 +112,14 @@ def _embed_bags(table, tokens, offsets, weights, scale, mean, out_dtype, keep):
     out = torch.empty((n_bags, table.shape[1]), dtype=out_dtype, device=dev)
     b = _bags(table, tokens, offsets, weights, scale, mean, out_dtype, inv)
     b.out, b.out_ld = out.data_ptr(), table.shape[1]
-    lib, ref = L.lib(), C.byref(b)
-
-    def work(stream):
-        ws = _workspace(lib.hanns_gpu_embed_bags_workspace_bytes(ref), dev, b)  # noqa: F841 (kept until enqueued)
-        _check(lib.hanns_gpu_embed_bags_device(ref, stream), "embed_bags")
-
-    _run(dev, work)
+    _run(dev, _embed_bags_call, b, dev)
     return out, inv
+
+
+def _embed_bags_call(stream, b, dev):
+    lib, ref = L.lib(), C.byref(b)
+    ws = _workspace(lib.hanns_gpu_embed_bags_workspace_bytes(ref), dev, b)  # noqa: F841 (kept until enqueued)
+    _check(lib.hanns_gpu_embed_bags_device(ref, stream), "embed_bags")
 
 
 class _EmbedBags(torch.autograd.Function):
@@ -245,19 +246,19 @@ def _token_logprobs(logits, tokens, top, temperature, near, keep):
     out = (torch.empty(n, dtype=f32, device=dev), torch.empty(n, dtype=f32, device=dev),
            torch.empty((n, top), dtype=torch.int64, device=dev), torch.empty((n, top), dtype=f32, device=dev),
            torch.empty((n, 4), dtype=f32, device=dev) if keep or near is not None else None)
-    t = _probs(logits, tokens, top, temperature, out)
-    lib, ref = L.lib(), C.byref(t)
-
-    def work(stream):
-        _check(lib.hanns_gpu_token_logprobs_device(ref, stream), "token_logprobs")
-        if near is not None:
-            ids, distances, values, weight, knn_temperature = near
-            _check(lib.hanns_gpu_neighbour_logprobs_device(
-                ref, ids.data_ptr(), distances.data_ptr(), ids.shape[-1], values.data_ptr(), values.numel(),
-                weight, knn_temperature, stream), "token_logprobs")
-
-    _run(dev, work)
+    _run(dev, _token_logprobs_call, _probs(logits, tokens, top, temperature, out), near)
     return out
+
+
+def _token_logprobs_call(stream, t, near):
+    lib, ref = L.lib(), C.byref(t)
+    rc = lib.hanns_gpu_token_logprobs_device(ref, stream)
+    if rc == 0 and near is not None:
+        ids, distances, values, weight, knn_temperature = near
+        rc = lib.hanns_gpu_neighbour_logprobs_device(
+            ref, ids.data_ptr(), distances.data_ptr(), ids.shape[-1], values.data_ptr(), values.numel(),
+            weight, knn_temperature, stream)
+    _check(rc, "token_logprobs")
 
 
 class _TokenLogprobs(torch.autograd.Function):
