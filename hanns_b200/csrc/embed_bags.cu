@@ -404,13 +404,13 @@ __global__ void __launch_bounds__(kSegmentThreads, blocks_of_sm(Packs, VE, true)
     sum_segment<T, TO, VE, Packs, false>(a, ln, batch[threadIdx.x >> 5], entries, seg, lo, hi, tile);
 }
 
-// Backward: one warp per (run, column tile), and behind those one per 32 table rows for the rows of
-// tokens without a run.  The same 150,001 tokens in f32, both gradients: 54 us, then 43 us for the
+// Backward: one warp per (run, column tile), and behind those one per 2^clear_log2 table rows for the
+// rows of tokens without a run.  The same 150,001 tokens in f32, both gradients: 54 us, then 43 us for the
 // pieces of tokens that occur more than 32 times (59 % of the positions).
 template <class T, class TO, int VE, int Packs, bool Dot>
 __global__ void __launch_bounds__(kSegmentThreads, blocks_of_sm(Packs, VE, false))
     runs_kernel(SumArgs a, SortedEntries entries, const Run* runs, const int32_t* n_runs, int64_t most_runs,
-                const uint32_t* touched) {
+                const uint32_t* touched, int clear_log2) {
     wait_for_previous();
     __shared__ Batch batch[kSegmentThreads / 32];
     const int64_t w = (int64_t)blockIdx.x * (kSegmentThreads / 32) + (threadIdx.x >> 5);
@@ -426,11 +426,11 @@ __global__ void __launch_bounds__(kSegmentThreads, blocks_of_sm(Packs, VE, false
         sum_segment<T, TO, VE, Packs, Dot>(a, ln, batch[threadIdx.x >> 5], entries, run.token, run.lo, run.hi, tile);
         return;
     }
-    const int64_t first = (w - most_runs * a.tiles) * 32;
+    const int64_t first = (w - most_runs * a.tiles) << clear_log2;
     if (first >= a.n_segments) return;
-    const int64_t left = a.n_segments - first;
-    uint32_t rows = ~touched[first / 32];
-    if (left < 32) rows &= (1u << left) - 1;
+    const int each = (int)min((int64_t)1 << clear_log2, a.n_segments - first);
+    uint32_t rows = ~touched[first / 32] >> (first & 31);
+    if (each < 32) rows &= (1u << each) - 1;
     const float2 zeros[Packs][(VE + 1) / 2] = {};
     for (; rows; rows &= rows - 1)
         for (int tile = 0; tile < a.tiles; ++tile)
@@ -1019,6 +1019,10 @@ unsigned grid_of(int64_t warps) {
     return (unsigned)((warps + of_block - 1) / of_block);
 }
 
+// Warps that clear the rows of tokens without a run: a row each until that is more than the SMs hold,
+// then up to 32 rows each.
+constexpr int64_t kMostClearing = 148 * 64;
+
 // Launches the kernels of the sums; `b` and `so` are the forward and the backward call's.
 template <class T, class TO, int VE, bool Dot, class Entries>
 void launch_sum(SumArgs& a, const Entries& entries, const BagSegments& bags, const SortArgs& so, cudaStream_t s) {
@@ -1043,9 +1047,11 @@ void launch_sum(SumArgs& a, const Entries& entries, const BagSegments& bags, con
                 launch_early(lookup_kernel<T, TO, VE, Packs>, grid, kSegmentThreads, 0, s, a, entries);
             }
         } else {
-            const int64_t warps = so.most_runs * a.tiles + (a.n_segments + 31) / 32;
+            int clear_log2 = 0;
+            while (clear_log2 < 5 && a.n_segments >> clear_log2 > kMostClearing) ++clear_log2;
+            const int64_t warps = so.most_runs * a.tiles + ((a.n_segments - 1) >> clear_log2) + 1;
             launch_early(runs_kernel<T, TO, VE, Packs, Dot>, grid_of(warps), kSegmentThreads, 0, s, a, entries, so.runs,
-                         so.n_runs, so.most_runs, so.touched);
+                         so.n_runs, so.most_runs, so.touched, clear_log2);
         }
     };
     if constexpr (several) {

@@ -146,15 +146,15 @@ def _embed_bags_grad(grad, table, tokens, offsets, weights, inv, scale, mean, ou
     d_table = torch.empty(table.shape, dtype=table.dtype, device=dev)
     d_weights = torch.empty(tokens.shape[0], dtype=torch.float32, device=dev) if want_weights else None
     b = _bags(table, tokens, offsets, weights, scale, mean, out_dtype, inv)
-    lib, ref = L.lib(), C.byref(b)
-
-    def work(stream):
-        ws = _workspace(lib.hanns_gpu_embed_bags_grad_workspace_bytes(ref), dev, b)  # noqa: F841 (kept until enqueued)
-        _check(lib.hanns_gpu_embed_bags_grad_device(ref, grad.data_ptr(), grad.stride(0), d_table.data_ptr(),
-                                                    table.shape[1], _ptr(d_weights), stream), "embed_bags")
-
-    _run(dev, work)
+    _run(dev, _embed_bags_grad_call, b, grad, d_table, d_weights)
     return d_table if want_table else None, d_weights
+
+
+def _embed_bags_grad_call(stream, b, grad, d_table, d_weights):
+    lib, ref = L.lib(), C.byref(b)
+    ws = _workspace(lib.hanns_gpu_embed_bags_grad_workspace_bytes(ref), d_table.device, b)  # noqa: F841 (kept until enqueued)
+    _check(lib.hanns_gpu_embed_bags_grad_device(ref, grad.data_ptr(), grad.stride(0), d_table.data_ptr(),
+                                                d_table.shape[1], _ptr(d_weights), stream), "embed_bags")
 
 
 def embed_bags(table, tokens, offsets=None, weights=None, *, scale: float = 1.0, mean: bool = False,
@@ -288,10 +288,14 @@ class _TokenLogprobs(torch.autograd.Function):
         ptr = logits.data_ptr()
         t = L.TokenLogprobs(_DTYPES[logits.dtype], top, n, vocab, logits.stride(0), temperature, 0, ptr,
                             tokens.data_ptr(), ptr, ptr, tt.data_ptr(), ptr, ctx.stats.data_ptr())
-        _run(logits.device, lambda stream: _check(L.lib().hanns_gpu_token_logprobs_grad_device(
-            C.byref(t), _ptr(g_logprobs), _ptr(g_entropy), _ptr(g_top), d.data_ptr(), vocab, stream),
-            "token_logprobs"))
+        _run(logits.device, _token_logprobs_grad_call, t, g_logprobs, g_entropy, g_top, d)
         return d, None, None, None
+
+
+def _token_logprobs_grad_call(stream, t, g_logprobs, g_entropy, g_top, d):
+    _check(L.lib().hanns_gpu_token_logprobs_grad_device(
+        C.byref(t), _ptr(g_logprobs), _ptr(g_entropy), _ptr(g_top), d.data_ptr(), d.shape[1], stream),
+        "token_logprobs")
 
 
 def token_logprobs(logits, tokens, *, top: int = 0, temperature: float = 1.0,

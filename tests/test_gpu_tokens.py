@@ -163,6 +163,16 @@ def test_sort_at_every_key_width(rows):
     check_bags(table, tokens.cuda(), offsets_of([n // 2, 0, n - n // 2]), torch.rand(n, generator=gen(2)).cuda())
 
 
+@pytest.mark.parametrize("rows", [31, 33, 9472, 9473, 18_945, 40_001, 160_007, 310_003])
+def test_rows_without_a_token_are_cleared(rows):
+    """At every number of rows a warp clears, with tokens in the first, the last and some rows."""
+    table = torch.randn(rows, 5, generator=gen(rows)).cuda()
+    tokens = torch.tensor([0, rows - 1, rows // 2, rows // 2, min(31, rows - 1), rows - 2]).cuda()
+    torch.full((rows, 5), math.nan, device="cuda")  # what the allocator may hand to the gradient
+    check_bags(table, tokens, None, None)
+    check_bags(table, tokens[:0], None, None)
+
+
 def test_lookup_shapes_and_types():
     table = torch.randn(50, 24, generator=gen(0)).to(BF16).cuda()
     for shape in ((), (1,), (7,), (3, 5), (2, 0, 4)):
