@@ -46,6 +46,10 @@ constexpr int blocks_of_sm(int packs, int ve, bool forward) {
 constexpr int kLookupPacks = 8;       // vectors of a lane in a lookup
 constexpr int kMaxBinBits = 9, kMaxBins = 1 << kMaxBinBits;
 constexpr int kSortItems = 4, kSortTile = kThreads * kSortItems;
+// Up to so many tiles each adds up the counts of those before it itself, without a scan kernel between.
+// A gradient of 8 tiles takes 23.4 us for 26.2 then, 16 tiles 38.3 for 40.6, 32 tiles 35.8 either
+// way, 64 tiles 46.2 for 44.0.
+constexpr int kFewTiles = 16;
 
 // ---------------------------------------------------------------- entries and segments
 // Position j of the tokens as the caller gave them.
@@ -84,17 +88,7 @@ struct BagSegments {
         lo = clamp_pos(offsets[i], 0, n_tokens);
         hi = clamp_pos(offsets[i + 1], lo, n_tokens);
     }
-    // The number of offsets that are at most p.
-    __device__ __forceinline__ int64_t starts_up_to(int64_t p) const {
-        int64_t a = 0, b = n_bags + 1;
-        while (a < b) {
-            const int64_t m = (a + b) >> 1;
-            if (offsets[m] <= p) a = m + 1;
-            else b = m;
-        }
-        return a;
-    }
-    // The same by a whole warp, a 32nd of the range a step.
+    // The number of offsets that are at most p, found by a whole warp: a 32nd of the range a step.
     __device__ __forceinline__ int64_t starts_up_to_by_warp(int64_t p) const {
         const int lane = threadIdx.x & 31;
         int64_t a = 0, n = n_bags + 1;  // the answer is in [a, a + n]
@@ -590,25 +584,42 @@ struct SortArgs {
     int32_t *list_counts, *n_runs;
     Run* runs;
     int64_t most_runs;
-    int32_t* hist;   // [bins][tiles]
+    int32_t* hist;   // [bins][tiles]; few tiles: [tiles][bins]
     int32_t* total;  // [bins]
 };
+
+// The lanes of the warp that hold the same digit: a ballot a bit, whose time does not grow with the
+// number of different digits as that of __match_any_sync does (one block's sort of 4,001 positions
+// 16 us for 19, a pass over 150,001 keys 4.4 for 4.9).
+template <int Bits>
+__device__ __forceinline__ uint32_t lanes_with(int d) {
+    uint32_t same = 0xffffffffu;
+#pragma unroll
+    for (int b = 0; b < Bits; ++b) {
+        const bool one = d >> b & 1;
+        const uint32_t ones = __ballot_sync(0xffffffffu, one);
+        same &= one ? ones : ~ones;
+    }
+    return same;
+}
 
 // The bags of a tile's positions, into bag[]: the offset at or before the tile is searched for,
 // those inside it are marked at their positions (the last of equal ones counts), and the largest
 // mark up to a position is its bag.
-__device__ void tile_bags(const BagSegments& bags, int64_t base, int32_t (&bag)[kSortTile], int32_t* warp_max) {
+template <int Threads>
+__device__ void tile_bags(const BagSegments& bags, int64_t base, int32_t* bag, int32_t* warp_max) {
+    constexpr int Tile = Threads * kSortItems;
     if (!bags.offsets) {
-        for (int i = threadIdx.x; i < kSortTile; i += kThreads) bag[i] = (int32_t)(base + i);
+        for (int i = threadIdx.x; i < Tile; i += Threads) bag[i] = (int32_t)(base + i);
         __syncthreads();
         return;
     }
     const int32_t before = (int32_t)bags.starts_up_to_by_warp(base);
-    for (int i = threadIdx.x; i < kSortTile; i += kThreads) bag[i] = before;
+    for (int i = threadIdx.x; i < Tile; i += Threads) bag[i] = before;
     __syncthreads();
-    for (int64_t k = before + threadIdx.x; k <= bags.n_bags; k += kThreads) {
+    for (int64_t k = before + threadIdx.x; k <= bags.n_bags; k += Threads) {
         const int64_t o = bags.offsets[k] - base;
-        if (o >= kSortTile) break;
+        if (o >= Tile) break;
         if (o > 0) atomicMax(&bag[o], (int32_t)(k + 1));
     }
     __syncthreads();
@@ -655,15 +666,16 @@ __global__ void __launch_bounds__(kThreads) sort_count_kernel(SortArgs a) {
     __shared__ int32_t bag[First ? kSortTile : 1], warp_max[kWarps];
     for (int b = threadIdx.x; b < a.bins; b += kThreads) count[b] = 0;
     const int64_t base = (int64_t)blockIdx.x * kSortTile;
-    int64_t token[kSortItems];
-    if constexpr (First) {
+    int64_t token[kSortItems];  // or the keys of a later pass; all are read before any is used
 #pragma unroll
-        for (int i = 0; i < kSortItems; ++i) {
-            const int64_t j = base + i * kThreads + threadIdx.x;
-            token[i] = j < a.n ? a.tokens[j] : -1;
-        }
+    for (int i = 0; i < kSortItems; ++i) {
+        const int64_t j = base + i * kThreads + threadIdx.x;
+        token[i] = -1;
+        if (j < a.n) token[i] = First ? a.tokens[j] : (int64_t)a.key_in[j];
+    }
+    if constexpr (First) {
         clear_runs(a);
-        tile_bags(a.bags, base, bag, warp_max);
+        tile_bags<kThreads>(a.bags, base, bag, warp_max);
     } else {
         __syncthreads();
     }
@@ -680,12 +692,15 @@ __global__ void __launch_bounds__(kThreads) sort_count_kernel(SortArgs a) {
             a.bag[j] = b;
             a.key_in[j] = key;
         } else {
-            key = a.key_in[j];
+            key = (uint32_t)token[i];
         }
         atomicAdd(&count[(key >> a.shift) & (a.bins - 1)], 1);
     }
     __syncthreads();
-    for (int b = threadIdx.x; b < a.bins; b += kThreads) a.hist[(int64_t)b * a.tiles + blockIdx.x] = count[b];
+    for (int b = threadIdx.x; b < a.bins; b += kThreads) {
+        const int64_t at = a.tiles > kFewTiles ? (int64_t)b * a.tiles + blockIdx.x : (int64_t)blockIdx.x * a.bins + b;
+        a.hist[at] = count[b];
+    }
 }
 
 // One warp per digit: its counts become the number of its keys in earlier tiles.
@@ -719,15 +734,47 @@ __global__ void __launch_bounds__(kThreads) sort_move_kernel(SortArgs a) {
     for (int b = threadIdx.x; b < kWarps * kMaxBins; b += kThreads) (&seen[0][0])[b] = 0;
     __syncthreads();
     const int64_t base = (int64_t)blockIdx.x * kSortTile + warp * (32 * kSortItems);
-    uint32_t key[kSortItems];
-    int32_t rank[kSortItems];
+    // all that is read, before it is used
+    uint32_t key[kSortItems], pos[kSortItems];
+    int32_t rank[kSortItems], bag[kSortItems];
+    float coef[kSortItems];
 #pragma unroll
     for (int i = 0; i < kSortItems; ++i) {
         const int64_t j = base + i * 32 + lane;
-        const bool in = j < a.n;
-        key[i] = in ? a.key_in[j] : 0;
+        key[i] = j < a.n ? a.key_in[j] : 0;
+        pos[i] = First ? (uint32_t)j : j < a.n ? a.pos_in[j] : 0;
+    }
+    // keys of digits b0 and b0 + 1 in all tiles and in those before this one
+    // (two digits per thread: bins <= 2 * kThreads)
+    const int b0 = threadIdx.x * 2;
+    int32_t all[2] = {}, earlier[2] = {};
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        if (b0 + q >= a.bins) continue;
+        if (a.tiles > kFewTiles) {
+            all[q] = a.total[b0 + q];
+            earlier[q] = a.hist[(int64_t)(b0 + q) * a.tiles + blockIdx.x];
+        } else {
+#pragma unroll 8
+            for (int t = 0; t < a.tiles; ++t) {
+                const int32_t c = a.hist[t * a.bins + b0 + q];
+                all[q] += c;
+                if (t < (int)blockIdx.x) earlier[q] += c;
+            }
+        }
+    }
+    if constexpr (Last) {
+#pragma unroll
+        for (int i = 0; i < kSortItems; ++i) bag[i] = base + i * 32 + lane < a.n ? a.bag[pos[i]] : -1;
+#pragma unroll
+        for (int i = 0; i < kSortItems; ++i)
+            coef[i] = base + i * 32 + lane < a.n ? entry_factor(a, pos[i], bag[i]) : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < kSortItems; ++i) {
+        const bool in = base + i * 32 + lane < a.n;
         const int d = (key[i] >> a.shift) & (a.bins - 1);
-        const uint32_t peers = __match_any_sync(0xffffffffu, in ? d : -1);
+        const uint32_t peers = lanes_with<kMaxBinBits>(d) & __ballot_sync(0xffffffffu, in);
         rank[i] = 0;
         if (in) rank[i] = seen[warp][d] + __popc(peers & ((1u << lane) - 1));
         __syncwarp();
@@ -735,12 +782,7 @@ __global__ void __launch_bounds__(kThreads) sort_move_kernel(SortArgs a) {
         __syncwarp();
     }
     __syncthreads();
-    // digits before this one, in all tiles: two digits per thread (bins <= 2 * kThreads)
-    int32_t t0 = 0, t1 = 0;
-    const int b0 = threadIdx.x * 2;
-    if (b0 < a.bins) t0 = a.total[b0];
-    if (b0 + 1 < a.bins) t1 = a.total[b0 + 1];
-    int32_t s = t0 + t1;
+    int32_t s = all[0] + all[1];
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
         const int32_t o = __shfl_up_sync(0xffffffffu, s, m);
@@ -748,17 +790,19 @@ __global__ void __launch_bounds__(kThreads) sort_move_kernel(SortArgs a) {
     }
     if (lane == 31) warp_sum[warp] = s;
     __syncthreads();
-    int32_t before = s - t0 - t1;
+    int32_t before = s - all[0] - all[1];  // keys of smaller digits
     for (int w = 0; w < warp; ++w) before += warp_sum[w];
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
         const int b = b0 + q;
         if (b < a.bins) {
-            int32_t at = before + (q ? t0 : 0) + a.hist[(int64_t)b * a.tiles + blockIdx.x];
+            int32_t at = before + (q ? all[0] : 0) + earlier[q], of_warp[kWarps];
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) of_warp[w] = seen[w][b];
+#pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                const int32_t c = seen[w][b];
                 seen[w][b] = at;
-                at += c;
+                at += of_warp[w];
             }
         }
     }
@@ -769,12 +813,10 @@ __global__ void __launch_bounds__(kThreads) sort_move_kernel(SortArgs a) {
         if (j >= a.n) continue;
         const int32_t to = seen[warp][(key[i] >> a.shift) & (a.bins - 1)] + rank[i];
         a.key_out[to] = key[i];
-        const uint32_t pos = First ? (uint32_t)j : a.pos_in[j];
-        a.pos_out[to] = pos;
-        if (Last) {
-            const int32_t bag = a.bag[pos];
-            a.src[to] = bag;
-            a.coef[to] = entry_factor(a, pos, bag);
+        a.pos_out[to] = pos[i];
+        if constexpr (Last) {
+            a.src[to] = bag[i];
+            a.coef[to] = coef[i];
         }
     }
 }
@@ -808,9 +850,11 @@ __global__ void __launch_bounds__(kThreads) sort_runs_kernel(SortArgs a, const u
 }
 
 // The whole sort and the list of runs for up to kSmallSort positions: one block, the keys in shared
-// memory, instead of seven launches whose work is nothing beside their starts (3,001 positions:
-// 17 us for 22 and the gaps between seven launches, the gradient's device time 43 us for 63).
+// memory, instead of five launches.  3,001 positions in 257 bags: 13.5 us, the whole gradient 19.5 us
+// on the device for 22 and 28 us of the host's for 37; at 4,001 positions the device takes 22.8 us
+// either way, beyond that several blocks are faster.
 constexpr int kSmallThreads = 1024, kSmallWarps = kSmallThreads / 32, kSmallItems = 4;
+static_assert(kSmallItems == kSortItems);  // tile_bags
 constexpr int kSmallSort = kSmallThreads * kSmallItems, kSmallBits = 8;
 constexpr int64_t kSmallRows = 1 << 20;  // bit maps that one block clears quickly
 
@@ -821,28 +865,34 @@ __global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(SortArgs a, i
     __shared__ uint16_t seen[kSmallWarps][1 << kSmallBits];  // a warp's keys per digit, then its first place
     __shared__ int32_t warp_sum[(1 << kSmallBits) / 32];
     __shared__ int32_t n_runs;
+    __shared__ int32_t warp_max[kSmallWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // places of this thread's items, in every pass
+    auto place = [&](int i) { return warp * (32 * kSmallItems) + i * 32 + lane; };
+    auto used = [&](int i) { return place(i) - lane < a.n; };  // alike in the warp; others take no part
     if (threadIdx.x < 2) a.list_counts[threadIdx.x] = 0;
     if (threadIdx.x == 0) n_runs = 0;
     for (int64_t i = threadIdx.x; i < (a.rows + 31) / 32; i += kSmallThreads) a.touched[i] = a.lengthy[i] = 0;
+    // the bags of the positions; the keys come to lie there later
+    int32_t* s_bag = reinterpret_cast<int32_t*>(s_key);
+    int64_t token[kSmallItems];
+#pragma unroll
+    for (int i = 0; i < kSmallItems; ++i) {
+        const int j = place(i);
+        token[i] = j < a.n ? a.tokens[j] : -1;
+    }
+    tile_bags<kSmallThreads>(a.bags, 0, s_bag, warp_max);
     uint32_t key[kSmallItems];
     uint16_t pos[kSmallItems];
-    // places of this thread's items, in every pass
-    auto place = [&](int i) { return warp * (32 * kSmallItems) + i * 32 + lane; };
 #pragma unroll
     for (int i = 0; i < kSmallItems; ++i) {
         const int j = place(i);
         pos[i] = (uint16_t)j;
         key[i] = 0xffffffffu;  // behind the last position
         if (j >= a.n) continue;
-        const int64_t t = a.tokens[j];
-        int32_t bag = -1;
-        if ((uint64_t)t < (uint64_t)a.rows) {
-            const int64_t starts = a.bags.offsets ? a.bags.starts_up_to(j) : j + 1;
-            if (starts <= a.bags.n_bags) bag = (int32_t)starts - 1;
-        }
+        const int32_t bag = (uint64_t)token[i] < (uint64_t)a.rows ? s_bag[j] : -1;
         a.bag[j] = bag;
-        key[i] = bag >= 0 ? (uint32_t)t : (uint32_t)a.rows;
+        key[i] = bag >= 0 ? (uint32_t)token[i] : (uint32_t)a.rows;
     }
     for (int p = 0; p < passes; ++p) {
         const int shift = p * kSmallBits;
@@ -852,8 +902,9 @@ __global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(SortArgs a, i
         int rank[kSmallItems];
 #pragma unroll
         for (int i = 0; i < kSmallItems; ++i) {
+            if (!used(i)) continue;
             const int d = (key[i] >> shift) & ((1 << kSmallBits) - 1);
-            const uint32_t peers = __match_any_sync(0xffffffffu, d);
+            const uint32_t peers = lanes_with<kSmallBits>(d);
             rank[i] = seen[warp][d] + __popc(peers & ((1u << lane) - 1));
             __syncwarp();
             if ((peers >> lane) == 1) seen[warp][d] += (uint16_t)__popc(peers);
@@ -861,12 +912,12 @@ __global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(SortArgs a, i
         }
         __syncthreads();
         int32_t total = 0, upto = 0;
+        uint16_t of_warp[kSmallWarps];  // this thread's digit
         if (threadIdx.x < 1 << kSmallBits) {
-            for (int w = 0; w < kSmallWarps; ++w) {
-                const int c = seen[w][threadIdx.x];
-                seen[w][threadIdx.x] = (uint16_t)total;
-                total += c;
-            }
+#pragma unroll
+            for (int w = 0; w < kSmallWarps; ++w) of_warp[w] = seen[w][threadIdx.x];
+#pragma unroll
+            for (int w = 0; w < kSmallWarps; ++w) total += of_warp[w];
             upto = total;
 #pragma unroll
             for (int m = 1; m < 32; m <<= 1) {
@@ -879,11 +930,16 @@ __global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(SortArgs a, i
         if (threadIdx.x < 1 << kSmallBits) {
             int32_t before = upto - total;
             for (int w = 0; w < warp; ++w) before += warp_sum[w];
-            for (int w = 0; w < kSmallWarps; ++w) seen[w][threadIdx.x] += (uint16_t)before;
+#pragma unroll
+            for (int w = 0; w < kSmallWarps; ++w) {
+                seen[w][threadIdx.x] = (uint16_t)before;
+                before += of_warp[w];
+            }
         }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < kSmallItems; ++i) {
+            if (!used(i)) continue;
             const int to = seen[warp][(key[i] >> shift) & ((1 << kSmallBits) - 1)] + rank[i];
             s_key[to] = key[i];
             s_pos[to] = pos[i];
@@ -891,20 +947,26 @@ __global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(SortArgs a, i
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < kSmallItems; ++i) {
+            if (!used(i)) continue;
             key[i] = s_key[place(i)];
             pos[i] = s_pos[place(i)];
         }
     }
+    int32_t bag[kSmallItems];
+    float coef[kSmallItems];
+#pragma unroll
+    for (int i = 0; i < kSmallItems; ++i) bag[i] = place(i) < a.n ? a.bag[pos[i]] : -1;
+#pragma unroll
+    for (int i = 0; i < kSmallItems; ++i) coef[i] = place(i) < a.n ? entry_factor(a, pos[i], bag[i]) : 0.0f;
 #pragma unroll
     for (int i = 0; i < kSmallItems; ++i) {
         const int at = place(i);
         const uint32_t k = key[i];
         const bool begins = k < a.rows && (at == 0 || s_key[at - 1] != k);
         if (at < a.n) {
-            const int32_t bag = a.bag[pos[i]];
             a.pos_out[at] = pos[i];
-            a.src[at] = bag;
-            a.coef[at] = entry_factor(a, pos[i], bag);
+            a.src[at] = bag[i];
+            a.coef[at] = coef[i];
         }
         int end = at + 1;
         if (begins) {
@@ -1141,7 +1203,7 @@ SortPlan sort_plan(int64_t rows, int64_t n) {
 template <bool First>
 void sort_pass(const SortArgs& a, bool last, cudaStream_t s) {
     launch_early(sort_count_kernel<First>, a.tiles, kThreads, 0, s, a);
-    launch_early(sort_scan_kernel, (a.bins + kWarps - 1) / kWarps, kThreads, 0, s, a);
+    if (a.tiles > kFewTiles) launch_early(sort_scan_kernel, (a.bins + kWarps - 1) / kWarps, kThreads, 0, s, a);
     if (last) launch_early(sort_move_kernel<First, true>, a.tiles, kThreads, 0, s, a);
     else launch_early(sort_move_kernel<First, false>, a.tiles, kThreads, 0, s, a);
 }
