@@ -1104,11 +1104,15 @@ void launch_probs(const hanns_token_logprobs_t* t, const ProbArgs& a, cudaStream
         return;
     }
     // A cluster's blocks share a row when the rows alone are few for the SMs, as long as each block
-    // still has a round of full loads: one row of 128,000 bf16 takes 8.5 us on eight blocks (one:
-    // 18.6); 300 rows of 50,257 with alternatives 13.7 us (on two blocks each 15.0).
+    // still has a round of full loads: one row of 128,000 bf16 takes 8 us on eight blocks (one:
+    // 18.6), 222 rows 17.4 on four (two: 21.5), 300 rows 23.5 on two (one: 33.5).  Up to six blocks an
+    // SM: clusters do not fill the eight places of every SM, and those left over wait (296 rows on
+    // four blocks 26.2, on two 23.1).  The alternatives of all blocks have a thread each to join
+    // them (100 rows of 50,257 with 20: 13.4 us on four blocks, 17.2 on eight).
     int parts = 1;
-    const int64_t want = 4 * sm_count();
-    while (parts < kMaxCluster && t->n * parts * 2 <= want && vectors / (parts * 2) >= kMaxThreads * kUnroll)
+    const int64_t want = 6 * sm_count();
+    while (parts < kMaxCluster && t->n * parts * 2 <= want && vectors / (parts * 2) >= kMaxThreads * kUnroll &&
+           parts * 2 * t->top <= kMaxThreads)
         parts *= 2;
     const int threads = kMaxThreads;
     cudaLaunchConfig_t cfg{};

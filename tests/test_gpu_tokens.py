@@ -392,6 +392,16 @@ def test_few_and_many_rows(dtype, n, vocab):
     check_probs(x, torch.randint(0, vocab, (n,), generator=gen(1)).cuda(), 20)
 
 
+@pytest.mark.parametrize("n, vocab, dtype", [(1, 128_000, BF16), (3, 40_000, F32), (111, 17_000, F16),
+                                             (222, 9_000, F32), (223, 20_000, BF16), (445, 9_000, BF16)])
+@pytest.mark.parametrize("top", [0, 1, 16, 17, 32])
+def test_shared_rows_with_any_alternatives(n, vocab, dtype, top):
+    """Rows shared by two, four and eight blocks and by none, on both sides of each rule."""
+    x = some_logits(n + top, n, vocab, dtype)
+    x[:, 3] = x[:, vocab - 2] = 14.0
+    check_probs(x, torch.randint(0, vocab, (n,), generator=gen(1)).cuda(), top)
+
+
 def special_rows(vocab, dtype):
     low = torch.finfo(dtype).min
     x = torch.randn(16, vocab, generator=gen(2)) * 2
