@@ -210,6 +210,19 @@ def test_positions_outside_every_bag():
     check_bags(table, tokens, torch.tensor([3, 5, 5, 9]).cuda(), w, mean=True)
 
 
+@pytest.mark.parametrize("n, empty", [(37, 33_000), (3000, 32_000), (3000, 36_000), (5000, 7000), (5000, 9500)])
+@pytest.mark.parametrize("place", ["front", "middle", "end"])
+def test_many_empty_bags(n, empty, place):
+    """On both sides of the number from which positions search for their bags; tokens in front of
+    the first bag and behind the last."""
+    cuts = np.arange(2, n - 1, 7)
+    at = {"front": cuts[0], "middle": cuts[len(cuts) // 2] + 1, "end": cuts[-1]}[place]
+    offsets = torch.from_numpy(np.sort(np.concatenate([cuts, np.full(empty, at)]))).cuda()
+    tokens, _ = random_bags(n, 50, [n])
+    table = torch.randn(50, 2, generator=gen(1)).cuda()
+    check_bags(table, tokens, offsets, torch.rand(n, generator=gen(2)).cuda(), mean=True)
+
+
 def test_padding_rows_are_not_read():
     """A NaN row that no counted token names does not spread."""
     table = torch.randn(4, 64).cuda()
