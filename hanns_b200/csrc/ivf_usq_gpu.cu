@@ -7,6 +7,7 @@
 #include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <fstream>
 #include <numeric>
 #include <stdexcept>
@@ -151,6 +152,7 @@ IvfUsqGpu::~IvfUsqGpu() {
     if (ev_scan_err_) cudaEventDestroy(ev_scan_err_);
     if (ev_fork_) cudaEventDestroy(ev_fork_);
     if (ev_join_) cudaEventDestroy(ev_join_);
+    if (ev_done_) cudaEventDestroy(ev_done_);
     if (aux_stream_) cudaStreamDestroy(aux_stream_);
     if (h_scan_err_) cudaFreeHost(h_scan_err_);
     if (copy_stream_) cudaStreamDestroy(copy_stream_);
@@ -164,6 +166,7 @@ void IvfUsqGpu::ensure_stream() {
         HANNS_CUDA_OK(cudaStreamCreateWithFlags(&aux_stream_, cudaStreamNonBlocking));
         HANNS_CUDA_OK(cudaEventCreateWithFlags(&ev_fork_, cudaEventDisableTiming));
         HANNS_CUDA_OK(cudaEventCreateWithFlags(&ev_join_, cudaEventDisableTiming));
+        HANNS_CUDA_OK(cudaEventCreateWithFlags(&ev_done_, cudaEventDisableTiming));
         for (auto& sl : ring_) {
             for (auto& e : sl.aux) HANNS_CUDA_OK(cudaEventCreate(&e));
             for (auto& e : sl.kt) HANNS_CUDA_OK(cudaEventCreate(&e));
@@ -177,6 +180,26 @@ void IvfUsqGpu::ensure_stream() {
         *h_scan_err_ = 0;
         HANNS_CUDA_OK(cudaDeviceGetAttribute(&sm_count_, cudaDevAttrMultiProcessorCount, device_));
     }
+}
+
+IvfUsqGpu::InOrder::InOrder(IvfUsqGpu& index, cudaStream_t s)
+    : index(index), s(s), captured(false), exceptions(std::uncaught_exceptions()) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    HANNS_CUDA_OK(cudaStreamIsCapturing(s, &status));
+    captured = status != cudaStreamCaptureStatusNone;
+    if (!captured) HANNS_CUDA_OK(cudaStreamWaitEvent(s, index.ev_done_, 0));
+}
+
+IvfUsqGpu::InOrder::~InOrder() {
+    if (captured) return;
+    if (std::uncaught_exceptions() > exceptions) {
+        // the call ended before it joined them itself
+        for (cudaStream_t own : {index.aux_stream_, index.copy_stream_}) {
+            cudaEventRecord(index.ev_join_, own);
+            cudaStreamWaitEvent(s, index.ev_join_, 0);
+        }
+    }
+    cudaEventRecord(index.ev_done_, s);
 }
 
 void IvfUsqGpu::check_supported() const {
@@ -323,6 +346,7 @@ void IvfUsqGpu::upload_rotation_centroid() {
 void IvfUsqGpu::import_artifact(const void* art_) {
     const auto* a = static_cast<const hanns_ivf_usq_artifact_t*>(art_);
     DeviceGuard g(device_);
+    const InOrder order(*this, stream_);
     if (a->dim != dim_ || a->nbits != nbits_ || a->nlist != nlist_ || a->padded_dim != D_)
         throw std::invalid_argument("artifact shape does not match the index");
     metric_ = a->metric;
@@ -388,6 +412,7 @@ void IvfUsqGpu::export_artifact(void* out_) const {
 // ---------------------------------------------------------------- train / add
 void IvfUsqGpu::train(const float* h_data, int64_t n, int kmeans_iters, uint64_t kmeans_seed) {
     DeviceGuard g(device_);
+    const InOrder order(*this, stream_);
     if (n < nlist_) throw std::invalid_argument("training data too small: n < nlist");
     DevBuf<float> x;
     h2d(x, h_data, (size_t)n * dim_, stream_);
@@ -487,6 +512,7 @@ void IvfUsqGpu::train(const float* h_data, int64_t n, int kmeans_iters, uint64_t
 
 void IvfUsqGpu::add(const float* h_data, int64_t n, const int64_t* h_ids) {
     DeviceGuard g(device_);
+    const InOrder order(*this, stream_);
     if (!trained_) throw std::invalid_argument("index not trained, call train() first");
     check_int_rerank("GPU encoder");
     if (n <= 0) return;
@@ -609,6 +635,7 @@ void shard_owners(const int64_t* sizes, int nlist, int world, int32_t* owner) {
 
 void IvfUsqGpu::shard(int rank, int world) {
     DeviceGuard g(device_);
+    const InOrder order(*this, stream_);
     if (world < 1 || rank < 0 || rank >= world) throw std::invalid_argument("bad rank/world");
     std::vector<int64_t> sizes(nlist_);
     for (int l = 0; l < nlist_; ++l) sizes[l] = h_list_off_[l + 1] - h_list_off_[l];
@@ -1028,6 +1055,7 @@ void IvfUsqGpu::search_device(const float* d_queries, int64_t nq, const SearchOp
                               int64_t* d_ids, float* d_dists, int64_t* d_counts, uint64_t* d_keys,
                               cudaStream_t stream) {
     DeviceGuard g(device_);
+    const InOrder order(*this, stream ? stream : stream_);
     run_search(d_queries, nullptr, nq, opt, d_ids, d_dists, d_counts, d_keys, stream);
     if (!stream) {
         HANNS_CUDA_OK(cudaStreamSynchronize(stream_));
@@ -1171,6 +1199,7 @@ void IvfUsqGpu::rerank_rows_device(const float* d_queries, int64_t nq, const int
     check_int_rerank("rerank_rows");
     if (nq <= 0 || m <= 0) throw std::invalid_argument("empty rerank request");
     cudaStream_t s = stream ? stream : stream_;
+    const InOrder order(*this, s);
     const int G = D_ / 4;
     w_qrot_.reserve((size_t)nq * D_);
     w_qp_.reserve(nq);
@@ -1208,6 +1237,7 @@ void IvfUsqGpu::prepare_device(const float* d_queries, int64_t nq, int nprobe, Q
     if (nq <= 0) throw std::invalid_argument("query dimension mismatch");
     if (!st.probes || !st.qp || !st.lut || !st.q_i8p) throw std::invalid_argument("null query state");
     cudaStream_t s = stream ? stream : stream_;
+    const InOrder order(*this, s);
     nprobe = std::max(1, std::min(nprobe, nlist_));
     if (!st.q_i8n) {
         w_qi8n_.reserve((size_t)nq * D_);
@@ -1230,6 +1260,7 @@ void IvfUsqGpu::search_prepared_device(int64_t nq, const SearchOptions& opt, Que
     if (nq <= 0) throw std::invalid_argument("query dimension mismatch");
     if (!st.probes || !st.qp || !st.lut || !st.q_i8p) throw std::invalid_argument("null query state");
     cudaStream_t s = stream ? stream : stream_;
+    const InOrder order(*this, s);
     const int k = std::max(opt.k, 1);
     const int nprobe = std::max(1, std::min(opt.nprobe, nlist_));
     const int G = D_ / 4;
@@ -1259,6 +1290,7 @@ void IvfUsqGpu::search_host(const float* h_queries, int64_t nq, const SearchOpti
                             const uint64_t* h_bitsets, const int32_t* h_query_bitset,
                             int64_t* h_ids, float* h_dists, int64_t* h_counts) {
     DeviceGuard g(device_);
+    const InOrder order(*this, stream_);
     SearchOptions opt = opt_in;
     const int k = std::max(opt.k, 1);
     opt.k = k;
@@ -1357,6 +1389,7 @@ void IvfUsqGpu::debug_candidates(const float* h_queries, int64_t nq, const Searc
 void IvfUsqGpu::debug_query(const float* h_queries, int64_t nq, int nprobe, int32_t* probes,
                             float* q_rot, int8_t* q_i8, int8_t* lut, float* scalars) {
     DeviceGuard g(device_);
+    const InOrder order(*this, stream_);
     if (!trained_) throw std::invalid_argument("index not trained");
     nprobe = std::max(1, std::min(nprobe, nlist_));
     const int G = D_ / 4;
@@ -1432,6 +1465,7 @@ void IvfUsqGpu::save(const std::string& path) const {
 
 void IvfUsqGpu::load(const std::string& path) {
     DeviceGuard g(device_);
+    const InOrder order(*this, stream_);
     std::ifstream f(path, std::ios::binary);
     if (!f) throw std::runtime_error("cannot open " + path);
     char magic[8];

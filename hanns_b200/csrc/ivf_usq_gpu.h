@@ -163,6 +163,21 @@ class IvfUsqGpu {
     void upload_rotation_centroid();
     void rebuild_fastscan();
     void ensure_stream();
+    // Every call that reads or writes the search workspace or changes the stored rows holds one
+    // of these: the handle's buffers are shared by its calls whatever streams they are on, so
+    // `s` first waits for the work of the call before this one, and when the call ends (with
+    // an error, too) all that it enqueued on the handle's own streams is joined to `s`, for the
+    // next call to wait for.  Calls being captured into a graph are ordered by their replays.
+    struct InOrder {
+        InOrder(IvfUsqGpu& index, cudaStream_t s);
+        ~InOrder();
+        InOrder(const InOrder&) = delete;
+        InOrder& operator=(const InOrder&) = delete;
+        IvfUsqGpu& index;
+        cudaStream_t s;
+        bool captured;
+        int exceptions;
+    };
     // d_q: device query rows.  h_q (nullable): host rows to upload into d_q first, in chunks
     // on copy_stream_ that overlap the per-query stages of the preceding chunk.
     void search_batch(const float* d_q, const float* h_q, int64_t nb, const SearchOptions& opt,
@@ -245,6 +260,7 @@ class IvfUsqGpu {
     cudaStream_t copy_stream_ = nullptr;  // host->device query upload
     cudaStream_t aux_stream_ = nullptr;   // rotation + query state, beside the coarse step
     cudaEvent_t ev_fork_ = nullptr, ev_join_ = nullptr;
+    cudaEvent_t ev_done_ = nullptr;  // the last call's work (InOrder)
 
     static constexpr int kMaxUploadChunks = 8;
     cudaEvent_t ev_up_[kMaxUploadChunks] = {};

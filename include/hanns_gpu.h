@@ -14,7 +14,10 @@
  *
  * Every call returns NULL / an error code on failure and never aborts the process;
  * hanns_gpu_last_error() describes the last failure of the calling thread.
- * Concurrent calls on one handle are serialised by the handle (one CUDA stream each).
+ * Calls on one handle are serialised by the handle: on the host by a mutex, on the device in
+ * the order in which they were made, whatever streams they were given (the handle's buffers
+ * are one call's after the other's).  A call that is captured into a graph is not: its
+ * replays must not overlap other calls on the handle.
  */
 #ifndef HANNS_GPU_H
 #define HANNS_GPU_H
