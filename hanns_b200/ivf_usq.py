@@ -266,10 +266,14 @@ class IvfUsqIndex:
                 self._tensor_stream = torch.cuda.Stream(dev)
             run = self._tensor_stream
             run.wait_stream(cur)
-        self.search_device(queries.data_ptr(), queries.shape[0], k, nprobe, ids.data_ptr(),
-                           dists.data_ptr(), stream=run.cuda_stream)
-        if run is not cur:
-            cur.wait_stream(run)
+        try:
+            self.search_device(queries.data_ptr(), queries.shape[0], k, nprobe, ids.data_ptr(),
+                               dists.data_ptr(), stream=run.cuda_stream)
+        finally:
+            # also where a later part of the search failed: what was enqueued before it uses
+            # tensors that go back to the current stream's pool
+            if run is not cur:
+                cur.wait_stream(run)
         return ids, dists
 
     def _check_vectors(self, t, what: str):

@@ -110,3 +110,37 @@ def test_names_are_exported():
     with pytest.raises(AttributeError):
         hanns_b200.no_such_name
     assert Neighbours(None, None, None).weight == 0.25
+
+
+class FakeStream:
+    def __init__(self, handle):
+        self.cuda_stream, self.waited = handle, []
+
+    def wait_stream(self, other):
+        self.waited.append(other)
+
+
+@pytest.mark.parametrize("fails", [False, True])
+def test_the_current_stream_waits_for_a_search_that_failed(monkeypatch, fails):
+    """Streams and the search are stand-ins: a search may fail after parts of it were enqueued."""
+    from hanns_b200 import IvfUsqConfig, IvfUsqIndex
+    cur, own = FakeStream(0), FakeStream(7)
+    empty = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *size, device, **kw: empty(*size, **kw))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda dev: cur)
+    monkeypatch.setattr(torch.cuda, "Stream", lambda dev: own)
+    idx = IvfUsqIndex.__new__(IvfUsqIndex)
+    idx.config, idx.device, idx._h = IvfUsqConfig(4, 1, 8), 0, None
+
+    def search_device(*args, stream):
+        assert stream == 7 and own.waited == [cur] and not cur.waited
+        if fails:
+            raise RuntimeError("out of memory")
+
+    monkeypatch.setattr(idx, "search_device", search_device, raising=False)
+    if fails:
+        with pytest.raises(RuntimeError, match="out of memory"):
+            idx._search_tensors(torch.zeros(2, 4), 3, 1)
+    else:
+        idx._search_tensors(torch.zeros(2, 4), 3, 1)
+    assert cur.waited == [own]
