@@ -140,6 +140,8 @@ IvfUsqGpu::IvfUsqGpu(int dim, int nlist, int nbits, int metric, uint64_t rotatio
 
 IvfUsqGpu::~IvfUsqGpu() {
     cudaSetDevice(device_);
+    // calls on a stream return once enqueued: their last one still writes the pinned error code
+    if (ev_done_) cudaEventSynchronize(ev_done_);
     for (auto& sl : ring_) {
         for (auto& e : sl.ev)
             if (e) cudaEventDestroy(e);

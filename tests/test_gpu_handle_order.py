@@ -149,3 +149,18 @@ def test_prepared_search_and_rerank_behind_a_search_in_flight(index):
         results.append([out, *state])
     assert same(got, want)
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("own_stream", [False, True])
+def test_an_index_freed_behind_a_search_in_flight(own_stream):
+    import torch
+    first = batch(1, 30_000)
+    want = alone(make_index(8000), first)
+    idx = make_index(8000)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream() if own_stream else None):
+        got = idx.search_tokens(*first, request())
+        idx.close()
+    make_index(1000)  # takes what the index gave back
+    torch.cuda.synchronize()
+    assert same(got, want)
