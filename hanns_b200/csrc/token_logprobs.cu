@@ -844,7 +844,10 @@ __global__ void __launch_bounds__(kGradThreads, 12) logprobs_grad_kernel(GradArg
             for (int k = 0; k < VE; ++k) out[e + k] = d.v[k];
         }
     };
-    if (!live || row_needs_differences<T>(st.x, a.c)) {
+    // a 16-bit element at the floor has 2^y = 0, which slope y must not turn into NaN (a large gradient of
+    // the entropy, a low temperature); exponents of f32 logits and those from differences are clamped
+    const bool steep = sizeof(T) == 2 && !(fabsf(floor_of<T>() * rg.c * rg.slope) < 1e37f);
+    if (!live || steep || row_needs_differences<T>(st.x, a.c)) {
         for (int j = b0 + threadIdx.x; j < b1; j += kGradThreads) {
             const Pack<T, VE> p = view.body[j];
             Pack<T, VE> d;

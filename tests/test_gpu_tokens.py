@@ -906,3 +906,29 @@ def test_training_step_of_a_token_encoder():
     (-lp.gather(1, given.cpu()[:, None]).sum() + 0.1 * (lp.exp() * lp).sum()).backward()
     # f32 logits and gradients: a few hundred roundings of values near 1
     close(got, ref.grad, 512 * U * (1 + ref.grad.abs()), "d_table")
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("vocab", [300, 9001])
+@pytest.mark.parametrize("temperature, g_entropy", [(0.01, 65536.0), (1.0, 2.0 ** 30), (1e-5, 1.0)])
+def test_masked_logits_have_no_gradient_however_large_the_entropys(dtype, vocab, temperature, g_entropy):
+    """A scaled loss's gradient of the entropy times a masked element's exponent is out of f32's range."""
+    x = some_logits(vocab, 3, vocab, dtype, scale=0.01)
+    x[:, 1::2] = -math.inf
+    x = x.requires_grad_()
+    r = token_logprobs(x, torch.tensor([0, 2, 4]).cuda(), temperature=temperature)
+    d, = torch.autograd.grad(r.entropy, x, torch.full((3,), g_entropy).cuda())
+    assert (d[:, 1::2] == 0).all()
+    if dtype != F16:  # (out of its range otherwise)
+        log_p, h, _, _, _ = prob_formula(x.detach(), temperature, torch.zeros(3))
+        p = log_p.exp()
+        inner = torch.where(p > 0, log_p.nan_to_num(0.0, 0.0, 0.0) + h[:, None], 0.0)
+        want = -p * g_entropy * inner / temperature
+        s, tol, tol_h = prob_tol(x.detach(), log_p, vocab, temperature)
+        size = p * g_entropy * (torch.where(log_p.isfinite(), -log_p, 0.0) + h[:, None] + 1)
+        tol_d = ((2 * s + 16 * U) * size + 4 * U * torch.where(log_p.isfinite(), -log_p, 0.0) * size
+                 + p * g_entropy * (tol_h[:, None] + tol.nan_to_num(0.0)) + 4 * U * size) / temperature
+        # a p below f32's smallest normal value 2^-126 is 0 on the GPU: its term is at most
+        # 2^-126 (126 ln 2 + H + 1) g / T, and H is at most ln 9001 < 10
+        lost = 2.0 ** -126 * 100 * g_entropy / temperature
+        close(d, want, tol_d.nan_to_num(0.0) + half_step(want, dtype) + lost, "d_logits")
