@@ -9,8 +9,9 @@
 //
 // logprobs_kernel reads the logits once: running maximum, sum and weighted sum per thread
 // (rescaled when the maximum grows).  Exponents are in powers of two, y = x c - R with
-// c = log2(e) / T and the reference R = m c as f32 rounds it: any R serves, since the same one
-// is taken off again, and y then has a single rounding.  For the alternatives each thread keeps
+// c = log2(e) / T and the reference R = m c as f32 rounds it: any R near m c serves, since the same
+// one is taken off again, and y then has a single rounding.  Logits so far from 0 that R's rounding
+// is many powers of two are summed from their differences (kNoRef).  For the alternatives each thread keeps
 // the maxima of its two largest rounds of loads; the `top`-th of the threads' maxima bounds the
 // row's `top`-th logit, and the few rounds that reach the bound are read again, from the L2.  A row
 // is one block's, or a cluster's when there are few rows: each block of the cluster then takes a
@@ -185,7 +186,10 @@ __device__ __forceinline__ void exponents(const Pack<float, 4>& p, float c, floa
     }
 }
 
-constexpr float kNoRef = -1e37f;  // below every reference that is used
+// References are kept to 2^27 in magnitude, where R's rounding moves y by 4 at most (at 1e10 it would
+// be 512 and 2^512 no f32).  A thread whose logits all lie below takes -2^27 itself: against that
+// they are 2^-200, which is right unless the whole row lies there.
+constexpr float kNoRef = -0x1p27f;
 
 // Largest element, NaN if there is one.
 __device__ __forceinline__ float pack_max(const Pack<float, 4>& p) {
@@ -231,14 +235,15 @@ template <class T>
 struct Running {
     float m = -INFINITY, ref;
     float2 s = make_float2(0.0f, 0.0f), u = make_float2(0.0f, 0.0f);
-    // masked elements before the first live one count as 2^0 against the floor, which a row's
+    // masked elements before the first live one may count as 2^0 against the floor, which a row's
     // maximum far above it makes nothing of
-    __device__ __forceinline__ explicit Running(float c) : ref(sizeof(T) == 2 ? floor_of<T>() * c : kNoRef) {}
+    __device__ __forceinline__ explicit Running(float c)
+        : ref(sizeof(T) == 2 ? fmaxf(floor_of<T>() * c, kNoRef) : kNoRef) {}
     // before elements of maximum vm are added
     __device__ __forceinline__ void reach(float vm, float c) {
         if (!(vm <= m)) {
             m = max_nan(vm, m);
-            const float to = sizeof(T) == 2 ? fmaxf(m, floor_of<T>()) * c : fmaxf(m * c, kNoRef), d = ref - to;
+            const float to = fmaxf((sizeof(T) == 2 ? fmaxf(m, floor_of<T>()) : m) * c, kNoRef), d = ref - to;
             rescale(d, s.x, u.x);
             rescale(d, s.y, u.y);
             ref = to;
@@ -257,13 +262,13 @@ struct Running {
     }
 };
 
-// Rows for which y = x c - R is not good enough: the reference or the floor overflows, or
-// masked elements at the floor would count (a maximum near the type's lowest value, a very
-// high or low temperature).  They are read again and summed from (x - m) c.
+// Rows for which y = x c - R is not good enough: the maximum is too far from 0 for a reference, the
+// floor overflows, or masked elements at the floor would count (a maximum near the type's lowest
+// value, a very high or low temperature).  They are read again and summed from (x - m) c.
 template <class T>
 __device__ __forceinline__ bool row_needs_differences(float m, float c) {
     bool bad = !(fabsf(m * c) < -kNoRef);
-    if (sizeof(T) == 2) bad = bad || !(floor_of<T>() * c > kNoRef) || !((floor_of<T>() - m) * c < -150.0f);
+    if (sizeof(T) == 2) bad = bad || !(floor_of<T>() * c > -1e37f) || !((floor_of<T>() - m) * c < -150.0f);
     return bad;
 }
 

@@ -932,3 +932,34 @@ def test_masked_logits_have_no_gradient_however_large_the_entropys(dtype, vocab,
         # 2^-126 (126 ln 2 + H + 1) g / T, and H is at most ln 9001 < 10
         lost = 2.0 ** -126 * 100 * g_entropy / temperature
         close(d, want, tol_d.nan_to_num(0.0) + half_step(want, dtype) + lost, "d_logits")
+
+
+# ------------------------------------------------------------------ logits of any size
+def large_rows(vocab, dtype):
+    """Masks of -1e9 to -1e30, rows of nothing else, and rows whose largest logit is as far from 0."""
+    g = gen(vocab)
+    x = torch.randn(12, vocab, generator=g) * 3
+    for r, low in enumerate((-1e9, -1e10, -1e12, -1e20, -1e30)):
+        x[r, : vocab - vocab // 4] = low
+    x[5] = -1e10
+    x[6] = -1e30
+    x[7] = -1e20 * (1 + torch.rand(vocab, generator=g))
+    x[8] = 1e10
+    x[8, ::3] -= 4096.0
+    x[9] = 3e12 * torch.rand(vocab, generator=g)
+    x[10, ::2] = 1e30
+    x[11, ::2] = -3e10
+    top = torch.finfo(dtype).max
+    return x.clamp(-top, top).to(dtype).cuda()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("vocab", [300, 3000, 70_001])
+@pytest.mark.parametrize("temperature", [1e-9, 1e-6, 1.0, 1e8])
+def test_logits_far_from_zero(dtype, vocab, temperature):
+    x = large_rows(vocab, dtype)
+    tokens = torch.randint(0, vocab, (12,), generator=gen(1)).cuda()
+    tokens[::2] = vocab - 1
+    # f16 gradients of 1 / temperature are out of range
+    check_probs(x, tokens, 5, temperature, train=dtype != F16 or temperature >= 1.0)
+    check_probs(x.repeat(60, 1), tokens.repeat(60), 0, temperature, train=False)
