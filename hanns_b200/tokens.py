@@ -6,8 +6,8 @@ token_logprobs  log probabilities of given tokens from logits, their entropy and
 
 Both go through the C ABI (hanns_gpu_embed_bags_*, hanns_gpu_token_logprobs_*,
 hanns_gpu_neighbour_logprobs_device), run on the current stream of the tensors' device,
-take their scratch from torch's allocator and are differentiable once.  Bad arguments raise
-ValueError, GPU failures RuntimeError.
+take their scratch from torch's allocator and are differentiable once, in reverse mode.  Bad
+arguments raise ValueError, GPU failures and derivatives that there are not RuntimeError.
 """
 from __future__ import annotations
 
@@ -16,6 +16,7 @@ from dataclasses import dataclass
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -93,6 +94,14 @@ def _once(what):
     """Gradients are enabled in a backward pass only where it is to be differentiated itself."""
     if torch.is_grad_enabled():
         raise RuntimeError(f"{what} can be differentiated once only")
+
+
+def _no_tangent(what, *tensors):
+    """Inputs of a forward-mode derivative need not require gradients: their results would come
+    without a tangent, which stands for zero."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
 # ---------------------------------------------------------------------------- embed_bags
@@ -197,6 +206,8 @@ def embed_bags(table, tokens, offsets=None, weights=None, *, scale: float = 1.0,
         _need(weights.numel() == tokens.numel(), "weights must have one value per token")
         if weights.dim() != 1 or not weights.is_contiguous():
             weights = weights.reshape(-1).contiguous()
+    if forward_ad._current_level >= 0:
+        _no_tangent("embed_bags", table, weights)
     scale = float(scale)
     _need(scale == scale and abs(scale) != float("inf"), "scale must be finite")
     args = _rows(table), tokens, offsets, weights, scale, bool(mean), out_dtype
@@ -337,6 +348,8 @@ def token_logprobs(logits, tokens, *, top: int = 0, temperature: float = 1.0,
         _need(values.dim() == 1, "neighbours.values must be one-dimensional")
         near = (ids, neighbours.distances.contiguous(), values, float(neighbours.weight),
                 float(neighbours.temperature))
+    if forward_ad._current_level >= 0:
+        _no_tangent("token_logprobs", logits, near and near[1])
     plain = logits.dim() == 2
     args = _rows(logits), tokens, top, temperature
     if not plain:

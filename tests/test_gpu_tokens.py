@@ -963,3 +963,27 @@ def test_logits_far_from_zero(dtype, vocab, temperature):
     # f16 gradients of 1 / temperature are out of range
     check_probs(x, tokens, 5, temperature, train=dtype != F16 or temperature >= 1.0)
     check_probs(x.repeat(60, 1), tokens.repeat(60), 0, temperature, train=False)
+
+
+# ------------------------------------------------------------------ derivatives there are not
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_are_refused(grad):
+    from torch.autograd import forward_ad as fw
+    table, w = torch.randn(6, 8).cuda().requires_grad_(grad), torch.rand(3).cuda().requires_grad_(grad)
+    tokens, offsets = torch.tensor([1, 2, 0]).cuda(), torch.tensor([0, 2, 3]).cuda()
+    x = torch.randn(3, 9).cuda().requires_grad_(grad)
+    near = Neighbours(tokens[:, None], torch.zeros(3, 1).cuda(), tokens)
+    with fw.dual_level():
+        def dual(t):
+            return fw.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: embed_bags(dual(table), tokens), lambda: embed_bags(dual(table), tokens, offsets),
+                     lambda: embed_bags(table, tokens, offsets, dual(w)), lambda: token_logprobs(dual(x), tokens, top=2),
+                     lambda: token_logprobs(dual(x.detach()), tokens, neighbours=near),
+                     lambda: token_logprobs(x.detach(), tokens, neighbours=Neighbours(
+                         tokens[:, None], dual(torch.zeros(3, 1).cuda()), tokens))):
+            with pytest.raises(RuntimeError, match="forward"):
+                call()
+        # inputs without a tangent are not refused
+        assert embed_bags(table, tokens, offsets, w).shape == (2, 8)
+        assert token_logprobs(x, tokens).logprobs.shape == (3,)
