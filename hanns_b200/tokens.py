@@ -275,17 +275,17 @@ def _token_logprobs_call(stream, t, near):
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top, temperature):
-        lp, h, tt, tl, ctx.stats = _token_logprobs(logits, tokens, top, temperature, None, True)
+        lp, h, tt, tl, stats = _token_logprobs(logits, tokens, top, temperature, None, True)
         ctx.mark_non_differentiable(tt)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, tokens, tt)
+        ctx.save_for_backward(logits, tokens, tt, stats)
         ctx.args = top, temperature
         return lp, h, tt, tl
 
     @staticmethod
     def backward(ctx, g_logprobs, g_entropy, _, g_top):
         _once("token_logprobs")
-        logits, tokens, tt = ctx.saved_tensors
+        logits, tokens, tt, stats = ctx.saved_tensors
         top, temperature = ctx.args
         if g_logprobs is not None:
             g_logprobs = g_logprobs.contiguous()
@@ -298,7 +298,7 @@ class _TokenLogprobs(torch.autograd.Function):
         # the forward call's outputs are not read: any non-null pointer stands for them
         ptr = logits.data_ptr()
         t = L.TokenLogprobs(_DTYPES[logits.dtype], top, n, vocab, logits.stride(0), temperature, 0, ptr,
-                            tokens.data_ptr(), ptr, ptr, tt.data_ptr(), ptr, ctx.stats.data_ptr())
+                            tokens.data_ptr(), ptr, ptr, tt.data_ptr(), ptr, stats.data_ptr())
         _run(logits.device, _token_logprobs_grad_call, t, g_logprobs, g_entropy, g_top, d)
         return d, None, None, None
 

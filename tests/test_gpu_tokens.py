@@ -987,3 +987,18 @@ def test_forward_mode_derivatives_are_refused(grad):
         # inputs without a tangent are not refused
         assert embed_bags(table, tokens, offsets, w).shape == (2, 8)
         assert token_logprobs(x, tokens).logprobs.shape == (3,)
+
+
+def test_backward_frees_what_the_forward_call_kept():
+    """All of it is saved as tensors: hooks see it, and it goes with a pass that keeps no graph."""
+    x = torch.randn(70_000, 8).cuda().requires_grad_()
+    tokens = torch.zeros(70_000, dtype=torch.long).cuda()
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(tuple(t.shape)) or t, lambda t: t):
+        r = token_logprobs(x, tokens)
+    assert (70_000, 4) in seen
+    held = torch.cuda.memory_allocated()
+    loss = r.logprobs.sum()
+    d, = torch.autograd.grad(loss, x)
+    del d, loss
+    assert torch.cuda.memory_allocated() <= held - 70_000 * 16
