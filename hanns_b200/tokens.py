@@ -105,11 +105,11 @@ def _no_tangent(what, *tensors):
 
 
 # ---------------------------------------------------------------------------- embed_bags
-def _bags(table, tokens, offsets, weights, scale, mean, out_dtype, inv_counts):
-    rows, dim = table.shape
+def _bags(shape, dtype, table, tokens, offsets, weights, scale, mean, out_dtype, inv_counts):
     n = tokens.shape[0]
-    return L.EmbedBags(_DTYPES[table.dtype], _DTYPES[out_dtype], dim, int(mean), rows, table.stride(0), n,
-                       n if offsets is None else offsets.shape[0] - 1, scale, 0, table.data_ptr(),
+    return L.EmbedBags(_DTYPES[dtype], _DTYPES[out_dtype], shape[1], int(mean), shape[0],
+                       0 if table is None else table.stride(0), n,
+                       n if offsets is None else offsets.shape[0] - 1, scale, 0, _ptr(table),
                        tokens.data_ptr(), _ptr(offsets), _ptr(weights), None, 0, _ptr(inv_counts), None, 0)
 
 
@@ -119,7 +119,7 @@ def _embed_bags(table, tokens, offsets, weights, scale, mean, out_dtype, keep):
     n_bags = tokens.shape[0] if offsets is None else offsets.shape[0] - 1
     inv = torch.empty(n_bags, dtype=torch.float32, device=dev) if mean and keep else None
     out = torch.empty((n_bags, table.shape[1]), dtype=out_dtype, device=dev)
-    b = _bags(table, tokens, offsets, weights, scale, mean, out_dtype, inv)
+    b = _bags(table.shape, table.dtype, table, tokens, offsets, weights, scale, mean, out_dtype, inv)
     b.out, b.out_ld = out.data_ptr(), table.shape[1]
     _run(dev, _embed_bags_call, b, dev)
     return out, inv
@@ -135,8 +135,9 @@ class _EmbedBags(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, tokens, offsets, weights, scale, mean, out_dtype):
         out, inv = _embed_bags(table, tokens, offsets, weights, scale, mean, out_dtype, True)
-        ctx.save_for_backward(table, tokens, offsets, weights, inv)
-        ctx.args = scale, mean, out_dtype
+        # only the weights' gradient reads the table, which may be updated in place otherwise
+        ctx.save_for_backward(table if ctx.needs_input_grad[3] else None, tokens, offsets, weights, inv)
+        ctx.args = table.shape, table.dtype, scale, mean, out_dtype
         return out
 
     @staticmethod
@@ -147,14 +148,14 @@ class _EmbedBags(torch.autograd.Function):
         return d_table, None, None, d_weights, None, None, None
 
 
-def _embed_bags_grad(grad, table, tokens, offsets, weights, inv, scale, mean, out_dtype, want_table,
-                     want_weights):
-    dev = table.device
+def _embed_bags_grad(grad, table, tokens, offsets, weights, inv, shape, dtype, scale, mean, out_dtype,
+                     want_table, want_weights):
+    dev = tokens.device
     grad = _rows(grad)
     # the weights' gradient is a by-product of the table's
-    d_table = torch.empty(table.shape, dtype=table.dtype, device=dev)
+    d_table = torch.empty(shape, dtype=dtype, device=dev)
     d_weights = torch.empty(tokens.shape[0], dtype=torch.float32, device=dev) if want_weights else None
-    b = _bags(table, tokens, offsets, weights, scale, mean, out_dtype, inv)
+    b = _bags(shape, dtype, table, tokens, offsets, weights, scale, mean, out_dtype, inv)
     _run(dev, _embed_bags_grad_call, b, grad, d_table, d_weights)
     return d_table if want_table else None, d_weights
 

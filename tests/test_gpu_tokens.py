@@ -1002,3 +1002,18 @@ def test_backward_frees_what_the_forward_call_kept():
     d, = torch.autograd.grad(loss, x)
     del d, loss
     assert torch.cuda.memory_allocated() <= held - 70_000 * 16
+
+
+def test_a_table_updated_before_the_backward_pass():
+    """The table's gradient does not read the table; the weights' does, and torch refuses it then."""
+    table, w = torch.randn(9, 8).cuda().requires_grad_(), torch.rand(5).cuda().requires_grad_()
+    tokens, offsets = torch.tensor([1, 8, 1, -1, 3]).cuda(), torch.tensor([0, 3, 5]).cuda()
+    g = torch.randn(2, 8).cuda()
+    want = torch.autograd.grad(embed_bags(table, tokens, offsets, w.detach(), mean=True), table, g)
+    out = embed_bags(table, tokens, offsets, w.detach(), mean=True)
+    both = embed_bags(table, tokens, offsets, w)
+    with torch.no_grad():
+        table.mul_(3.0)
+    assert torch.equal(torch.autograd.grad(out, table, g)[0], want[0])
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(both, [table, w], g)
