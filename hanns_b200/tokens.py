@@ -343,6 +343,8 @@ def token_logprobs(logits, tokens, *, top: int = 0, temperature: float = 1.0,
         ids = _ids(neighbours.ids, dev, "neighbours.ids")
         _on(neighbours.distances, dev, "neighbours.distances")
         _need(neighbours.distances.dtype == torch.float32, "neighbours.distances must be float32")
+        _need(not (neighbours.distances.requires_grad and torch.is_grad_enabled()),
+              "token_logprobs with neighbours is not differentiable: detach the distances")
         _need(ids.dim() >= 1 and ids.shape[:-1] == tokens.shape and ids.shape == neighbours.distances.shape,
               "neighbours.ids and .distances must be tokens.shape + (k,)")
         values = _ids(neighbours.values, dev, "neighbours.values")

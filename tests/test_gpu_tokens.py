@@ -1017,3 +1017,15 @@ def test_a_table_updated_before_the_backward_pass():
     assert torch.equal(torch.autograd.grad(out, table, g)[0], want[0])
     with pytest.raises(RuntimeError, match="inplace"):
         torch.autograd.grad(both, [table, w], g)
+
+
+def test_distances_with_gradients_are_refused():
+    x, t = torch.randn(3, 9).cuda(), torch.tensor([1, 2, 0]).cuda()
+    dist = torch.rand(3, 1).cuda().requires_grad_()
+    near = Neighbours(t[:, None], dist, t)
+    with pytest.raises(ValueError, match="distances"):
+        token_logprobs(x, t, neighbours=near)
+    with torch.no_grad():
+        got = token_logprobs(x, t, neighbours=near)
+    want = token_logprobs(x, t, neighbours=Neighbours(t[:, None], dist.detach(), t))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
