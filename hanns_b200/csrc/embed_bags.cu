@@ -1261,7 +1261,8 @@ struct GradSpace {
         sum.n_entries = b->n_tokens;
         take_lists(sum, ws);
         sort.list_counts = sum.lists.count;
-        sum.dot = ws.take<float>(b->weights ? n * most_tiles(b->dim) : 0);
+        // inner products of the weights' gradient, which needs the table
+        sum.dot = ws.take<float>(b->weights && b->table ? n * most_tiles(b->dim) : 0);
     }
 };
 

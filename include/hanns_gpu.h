@@ -417,7 +417,8 @@ int32_t hanns_gpu_embed_bags_device(const hanns_embed_bags_t* bags, void* stream
  * dim of the table's type, every row written) and, where there are weights, d_weights (may be
  * NULL; n_tokens, zero for positions that do not count).  A token's terms are added in the
  * order of its positions: results do not change from run to run.  `out` is not read; a mean
- * needs the forward call's inv_counts; table may be NULL when d_weights is. */
+ * needs the forward call's inv_counts; table may be NULL when d_weights is, in both calls
+ * (the workspace is then smaller where there are weights). */
 int64_t hanns_gpu_embed_bags_grad_workspace_bytes(const hanns_embed_bags_t* bags);
 int32_t hanns_gpu_embed_bags_grad_device(const hanns_embed_bags_t* bags, const void* grad,
                                          int64_t grad_ld, void* d_table, int64_t d_table_ld,

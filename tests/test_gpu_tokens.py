@@ -1029,3 +1029,23 @@ def test_distances_with_gradients_are_refused():
         got = token_logprobs(x, t, neighbours=near)
     want = token_logprobs(x, t, neighbours=Neighbours(t[:, None], dist.detach(), t))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_memory_of_a_gradient_of_the_table_alone():
+    """Weights without a gradient: the same table gradient, with no more memory than without weights."""
+    n, dim = 200_000, 256
+    table = torch.randn(1000, dim, generator=gen(0)).cuda().requires_grad_()
+    tokens = torch.randint(0, 1000, (n,), generator=gen(1)).cuda()
+    offsets, w = offsets_of([n // 4] * 4), torch.rand(n, generator=gen(2)).cuda()
+    g = torch.randn(4, dim, generator=gen(3)).cuda()
+    peak, grads = {}, {}
+    for name, weights, leaves in (("none", None, [table]), ("alone", w, [table]),
+                                  ("both", w.clone().requires_grad_(), None)):
+        out = embed_bags(table, tokens, offsets, weights)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        grads[name] = torch.autograd.grad(out, leaves or [table, weights], g)[0]
+        peak[name] = torch.cuda.max_memory_allocated() - before
+    assert torch.equal(grads["alone"], grads["both"])
+    assert peak["alone"] == peak["none"] and peak["both"] >= peak["alone"] + 4 * n * dim // 32

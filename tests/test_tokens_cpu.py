@@ -144,3 +144,18 @@ def test_the_current_stream_waits_for_a_search_that_failed(monkeypatch, fails):
     else:
         idx._search_tensors(torch.zeros(2, 4), 3, 1)
     assert cur.waited == [own]
+
+
+def test_the_tables_gradient_alone_needs_no_room_for_inner_products():
+    lib = L.lib()
+    n, dim = 100_000, 768
+    kw = dict(n_tokens=n, n_bags=10, dim=dim, ld=dim, out_ld=dim)
+    plain = lib.hanns_gpu_embed_bags_grad_workspace_bytes(C.byref(bags(**kw)))
+    alone = lib.hanns_gpu_embed_bags_grad_workspace_bytes(C.byref(bags(weights=256, table=None, **kw)))
+    both = lib.hanns_gpu_embed_bags_grad_workspace_bytes(C.byref(bags(weights=256, **kw)))
+    assert alone == plain
+    assert both - alone >= n * 4 * dim // 32
+    # and asks for no more
+    b = bags(weights=256, table=None, workspace=256, workspace_bytes=alone - 1, **kw)
+    assert lib.hanns_gpu_embed_bags_grad_device(C.byref(b), 256, dim, 256, dim, None, None) == 2
+    assert "too small" in L.last_error()
