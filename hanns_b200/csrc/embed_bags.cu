@@ -649,9 +649,10 @@ __device__ void tile_bags(const BagSegments& bags, int64_t base, int32_t* bag, i
     for (int i = threadIdx.x; i < Tile; i += Threads) bag[i] = before;
     __syncthreads();
 #pragma unroll 4
-    for (int32_t k = before + threadIdx.x; k < after; k += Threads) {
+    // (unsigned: k may pass 2^31 in its last step)
+    for (uint32_t k = (uint32_t)before + threadIdx.x; k < (uint32_t)after; k += Threads) {
         const int64_t o = bags.offsets[k] - base;
-        if (o > 0 && o < Tile) atomicMax(&bag[o], k + 1);
+        if (o > 0 && o < Tile) atomicMax(&bag[o], (int32_t)k + 1);
     }
     __syncthreads();
     int32_t v[kSortItems];

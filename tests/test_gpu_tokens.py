@@ -1049,3 +1049,17 @@ def test_memory_of_a_gradient_of_the_table_alone():
         peak[name] = torch.cuda.max_memory_allocated() - before
     assert torch.equal(grads["alone"], grads["both"])
     assert peak["alone"] == peak["none"] and peak["both"] >= peak["alone"] + 4 * n * dim // 32
+
+
+def test_as_many_bags_as_there_may_be():
+    """2^31 - 2 of them, three tokens in the last three: indexes of offsets reach 2^31 - 2."""
+    n = 2 ** 31 - 2
+    offsets = torch.zeros(n + 1, dtype=torch.long, device="cuda")
+    offsets[-3:] = torch.tensor([1, 2, 3]).cuda()
+    table = torch.tensor([[1.0], [2.0], [4.0], [8.0]]).to(BF16).cuda().requires_grad_()
+    tokens = torch.tensor([3, 1, 3]).cuda()
+    out = embed_bags(table, tokens, offsets)
+    assert out.shape == (n, 1) and out[-3:, 0].tolist() == [8.0, 2.0, 8.0]
+    assert not out.detach()[:-3].any()
+    g, = torch.autograd.grad(out, table, torch.full((1, 1), 3.0).to(BF16).cuda().expand(n, 1))
+    assert g[:, 0].tolist() == [0.0, 3.0, 0.0, 6.0]
