@@ -1210,6 +1210,15 @@ void check_bags(const hanns_embed_bags_t* b) {
     require(b->n_tokens >= 0 && b->n_tokens < 0x7fffffff, "embed_bags: n_tokens must be in [0, 2^31 - 1)");
     require(b->n_bags >= 0 && b->n_bags < 0x7fffffff, "embed_bags: n_bags must be in [0, 2^31 - 1)");
     require(b->offsets || b->n_bags == b->n_tokens, "embed_bags: without offsets each token is its own bag");
+    require(aligned(b->tokens, 8) && aligned(b->offsets, 8), "embed_bags: misaligned tokens or offsets");
+    require(aligned(b->weights, 4) && aligned(b->inv_counts, 4), "embed_bags: misaligned weights or inv_counts");
+    require(aligned(b->table, dtype_bytes(b->dtype)), "embed_bags: misaligned table");
+}
+
+// Rows that are read may overlap (a broadcast row is `ld` 0), rows that are written may not.
+void check_read(int64_t ld) { require(ld >= 0, "embed_bags: rows must not run backwards"); }
+void check_written(int64_t rows, int64_t ld, int dim) {
+    require(rows <= 1 || ld >= dim, "embed_bags: output rows overlap");
 }
 
 void check_workspace(size_t need, const void* p, int64_t have) {
@@ -1294,6 +1303,9 @@ extern "C" int32_t hanns_gpu_embed_bags_device(const hanns_embed_bags_t* b, void
         check_bags(b);
         if (b->n_bags == 0) return;
         require(b->table && b->out && (b->tokens || b->n_tokens == 0), "embed_bags: null table, tokens or out");
+        require(aligned(b->out, dtype_bytes(b->out_dtype)), "embed_bags: misaligned out");
+        check_read(b->ld);
+        check_written(b->n_bags, b->out_ld, b->dim);
         check_workspace((size_t)hanns_gpu_embed_bags_workspace_bytes(b), b->workspace, b->workspace_bytes);
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         SumArgs a{};
@@ -1342,6 +1354,12 @@ extern "C" int32_t hanns_gpu_embed_bags_grad_device(const hanns_embed_bags_t* b,
         require(!b->mean || b->inv_counts || b->n_bags == 0, "embed_bags: a mean's gradient needs inv_counts");
         require(!d_weights || (b->table && b->weights),
                 "embed_bags: the weights' gradient needs the table and the weights");
+        require(aligned(grad, dtype_bytes(b->out_dtype)) && aligned(d_table, dtype_bytes(b->dtype)) &&
+                    aligned(d_weights, 4),
+                "embed_bags: misaligned gradient");
+        check_read(grad_ld);
+        if (d_weights) check_read(b->ld);
+        check_written(b->rows, d_table_ld, b->dim);
         check_workspace((size_t)hanns_gpu_embed_bags_grad_workspace_bytes(b), b->workspace, b->workspace_bytes);
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         const SortPlan sp = sort_plan(b->rows, b->n_tokens);

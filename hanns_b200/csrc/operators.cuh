@@ -41,6 +41,9 @@ inline void require(bool ok, const char* what) {
     if (!ok) throw std::invalid_argument(what);
 }
 
+// A pointer that the kernels may read or write as elements of `bytes` bytes (null is another check's).
+inline bool aligned(const void* p, size_t bytes) { return (uintptr_t)p % bytes == 0; }
+
 // Kernels are started while the one before them in the stream comes to its end, and wait here for it
 // to have finished before they read or write anything.  (Every kernel waits, so that waiting for one
 // is waiting for all before it.)  The gradient of 150,001 tokens takes 121 us for 142 this way.

@@ -1089,9 +1089,16 @@ void check_probs(const hanns_token_logprobs_t* t) {
     require(t->temperature > 1e-30f && t->temperature < 1e30f, "token_logprobs: temperature must be positive and finite");
     if (t->n == 0) return;
     require(t->logits && t->tokens && t->logprobs && t->entropy, "token_logprobs: null logits, tokens or output");
-    require((uintptr_t)t->logits % dtype_bytes(t->dtype) == 0, "token_logprobs: misaligned logits");
+    require(aligned(t->logits, dtype_bytes(t->dtype)), "token_logprobs: misaligned logits");
+    require(t->ld >= 0, "token_logprobs: rows must not run backwards");
+    require(aligned(t->tokens, 8) && (t->top == 0 || aligned(t->top_tokens, 8)), "token_logprobs: misaligned tokens");
     require(t->top == 0 || (t->top_tokens && t->top_logprobs), "token_logprobs: null output of the alternatives");
-    require((uintptr_t)t->stats % 16 == 0, "token_logprobs: stats must be 16-byte aligned");
+    require(aligned(t->stats, 16), "token_logprobs: stats must be 16-byte aligned");
+}
+// Of the calls that write them.
+void check_outputs(const hanns_token_logprobs_t* t) {
+    require(t->n == 0 || (aligned(t->logprobs, 4) && aligned(t->entropy, 4) && (t->top == 0 || aligned(t->top_logprobs, 4))),
+            "token_logprobs: misaligned output");
 }
 
 // The launch rules count the SMs of a B200 (a launch is right on any number).
@@ -1172,6 +1179,7 @@ extern "C" int32_t hanns_gpu_token_logprobs_device(const hanns_token_logprobs_t*
     return hanns::operator_entry([&] {
         using namespace hanns;
         check_probs(t);
+        check_outputs(t);
         if (t->n == 0) return;
         ProbArgs a{};
         a.logits = t->logits;
@@ -1201,7 +1209,10 @@ extern "C" int32_t hanns_gpu_token_logprobs_grad_device(const hanns_token_logpro
         check_probs(t);
         if (t->n == 0) return;
         require(t->stats && d_logits, "token_logprobs: the gradient needs stats and an output");
-        require((uintptr_t)d_logits % dtype_bytes(t->dtype) == 0, "token_logprobs: misaligned gradient");
+        require(aligned(d_logits, dtype_bytes(t->dtype)), "token_logprobs: misaligned gradient");
+        require(aligned(g_logprobs, 4) && aligned(g_entropy, 4) && aligned(g_top, 4),
+                "token_logprobs: misaligned gradients of the outputs");
+        require(t->n <= 1 || d_ld >= t->vocab, "token_logprobs: the gradient's rows overlap");
         GradArgs a{};
         a.logits = t->logits;
         a.ld = t->ld;
@@ -1231,6 +1242,7 @@ extern "C" int32_t hanns_gpu_neighbour_logprobs_device(const hanns_token_logprob
     return hanns::operator_entry([&] {
         using namespace hanns;
         check_probs(t);
+        check_outputs(t);
         require(k >= 0 && k <= kMaxNeighbours, "neighbour_logprobs: k must be in [0, 1024]");
         require(weight >= 0.0f && weight <= 1.0f, "neighbour_logprobs: weight must be in [0, 1]");
         require(knn_temperature > 1e-30f && knn_temperature < 1e30f,
@@ -1238,6 +1250,8 @@ extern "C" int32_t hanns_gpu_neighbour_logprobs_device(const hanns_token_logprob
         if (t->n == 0 || k == 0 || n_values <= 0 || weight == 0.0f) return;
         require(t->stats, "neighbour_logprobs: the model's statistics (stats) are needed");
         require(d_ids && d_distances && d_values, "neighbour_logprobs: null ids, distances or values");
+        require(aligned(d_ids, 8) && aligned(d_distances, 4) && aligned(d_values, 8),
+                "neighbour_logprobs: misaligned ids, distances or values");
         NearArgs a{};
         a.logits = t->logits;
         a.ld = t->ld;

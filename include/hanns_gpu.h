@@ -382,7 +382,9 @@ int32_t hanns_gpu_coarse_probes_static(const float* d_queries, int64_t nq,
  * (cudaStream_t, NULL = the legacy default stream): a call returns once its work is enqueued,
  * allocates nothing and may be captured into a graph.  Scratch is the caller's, sized by
  * the matching *_workspace_bytes (-1 for bad arguments), 256-byte aligned; calls that may
- * run at the same time need workspaces of their own. */
+ * run at the same time need workspaces of their own.  Pointers must be aligned to their
+ * elements; rows that are read may overlap (a broadcast row is ld 0), rows that are written may
+ * not. */
 #define HANNS_DTYPE_F32 0
 #define HANNS_DTYPE_F16 1
 #define HANNS_DTYPE_BF16 2

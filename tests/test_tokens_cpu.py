@@ -159,3 +159,50 @@ def test_the_tables_gradient_alone_needs_no_room_for_inner_products():
     b = bags(weights=256, table=None, workspace=256, workspace_bytes=alone - 1, **kw)
     assert lib.hanns_gpu_embed_bags_grad_device(C.byref(b), 256, dim, 256, dim, None, None) == 2
     assert "too small" in L.last_error()
+
+
+@pytest.mark.parametrize("kw, what", [
+    (dict(table=258), "misaligned"), (dict(table=257, dtype=2), "misaligned"), (dict(tokens=260), "misaligned"),
+    (dict(offsets=260), "misaligned"), (dict(weights=258), "misaligned"), (dict(inv_counts=257, mean=1), "misaligned"),
+    (dict(out=258), "misaligned"), (dict(out=258, dtype=2), "misaligned"), (dict(ld=-8), "backwards"),
+    (dict(out_ld=7), "overlap"), (dict(out_ld=0), "overlap"), (dict(out_ld=-8), "overlap")])
+def test_embed_bags_refuses_what_its_kernels_cannot_address(kw, what):
+    b = bags(**{"n_tokens": 100_000, "workspace": 256, "workspace_bytes": 8, **kw})  # (refused anyway: too small)
+    assert L.lib().hanns_gpu_embed_bags_device(C.byref(b), None) == 2
+    assert what in L.last_error()
+
+
+def test_embed_bags_grad_refuses_what_its_kernels_cannot_address():
+    lib = L.lib()
+    for args, kw, what in [((258, 8, 256, 8, None), {}, "misaligned"), ((256, 8, 258, 8, None), {}, "misaligned"),
+                           ((256, 8, 256, 8, 258), dict(weights=256), "misaligned"),
+                           ((256, -8, 256, 8, None), {}, "backwards"), ((256, 8, 256, 7, None), {}, "overlap"),
+                           ((256, 8, 256, 8, 256), dict(weights=256, ld=-8), "backwards")]:
+        b = bags(**kw)  # (no workspace: refused anyway)
+        assert lib.hanns_gpu_embed_bags_grad_device(C.byref(b), *args, None) == 2
+        assert what in L.last_error()
+
+
+@pytest.mark.parametrize("kw, what", [
+    (dict(tokens=260), "misaligned"), (dict(logprobs=258), "misaligned"), (dict(entropy=257), "misaligned"),
+    (dict(top_tokens=260), "misaligned"), (dict(top_logprobs=258), "misaligned"), (dict(ld=-10), "backwards")])
+def test_token_logprobs_refuses_what_its_kernels_cannot_address(kw, what):
+    lib = L.lib()
+    for call in (lambda t: lib.hanns_gpu_token_logprobs_device(C.byref(t), None),
+                 lambda t: lib.hanns_gpu_neighbour_logprobs_device(C.byref(t), 256, 256, 4, 256, 9, 0.0, 1.0, None)):
+        assert call(probs(**kw)) == 2
+        assert what in L.last_error()
+
+
+def test_token_logprobs_grad_and_neighbours_refuse_what_their_kernels_cannot_address():
+    lib = L.lib()
+    for args, what in [((258, None, None, 256, 10), "misaligned"), ((None, 257, None, 256, 10), "misaligned"),
+                       ((None, None, 258, 256, 10), "misaligned"), ((256, None, None, 256, 9), "overlap"),
+                       ((256, None, None, 256, -10), "overlap")]:
+        t = probs()
+        assert lib.hanns_gpu_token_logprobs_grad_device(C.byref(t), *args, None) == 2
+        assert what in L.last_error()
+    for ids, dist, values in ((260, 256, 256), (256, 258, 256), (256, 256, 260)):
+        t = probs()
+        assert lib.hanns_gpu_neighbour_logprobs_device(C.byref(t), ids, dist, 4, values, 9, 0.5, 1.0, None) == 2
+        assert "misaligned" in L.last_error()
