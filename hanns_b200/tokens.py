@@ -183,7 +183,7 @@ def embed_bags(table, tokens, offsets=None, weights=None, *, scale: float = 1.0,
     out_dtype  the table's type (default) or float32, which IvfUsqIndex searches
 
     A token outside [0, rows) is not counted (-1 pads, as in search results); an empty bag
-    gives zeros; positions outside every bag are not read.  Sums are f32, rounded once.
+    gives zeros; positions outside every bag do not count.  Sums are f32, rounded once.
     Differentiable in table (a dense gradient) and weights; the gradients add a token's terms in
     the order of its positions and do not change from run to run.
     """

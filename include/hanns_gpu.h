@@ -393,7 +393,8 @@ int32_t hanns_gpu_coarse_probes_static(const float* d_queries, int64_t nq,
  * weights[j] * table[t_j], summed in f32, c_i = the bag's counted tokens for a mean, else 1.
  * A token outside [0, rows) is not counted and adds nothing; an empty bag's row is zero.
  * Bag i is tokens[offsets[i] .. offsets[i+1]), offsets ascending; positions outside every
- * bag are not read.  offsets NULL: every token is its own bag (n_bags = n_tokens). */
+ * bag do not count, but the gradient reads all n_tokens tokens and weights.  offsets NULL:
+ * every token is its own bag (n_bags = n_tokens). */
 typedef struct {
     int32_t dtype;     /* HANNS_DTYPE_* of the table */
     int32_t out_dtype; /* the table's type, or f32 */
