@@ -1063,3 +1063,62 @@ def test_as_many_bags_as_there_may_be():
     assert not out.detach()[:-3].any()
     g, = torch.autograd.grad(out, table, torch.full((1, 1), 3.0).to(BF16).cuda().expand(n, 1))
     assert g[:, 0].tolist() == [0.0, 3.0, 0.0, 6.0]
+
+
+# ------------------------------------------------------------------ inputs at their edges
+def test_weights_alone_have_a_gradient():
+    """A frozen table: the weights' gradient is the one that comes with the table's."""
+    for dtype, rows, n, dim in ((F32, 50, 300, 33), (BF16, 3000, 9001, 128)):
+        table = torch.randn(rows, dim, generator=gen(0)).to(dtype).cuda()
+        tokens, offsets = random_bags(1, rows, [n // 3, 0, n // 3, 5])
+        w = torch.rand(tokens.numel(), generator=gen(2)).cuda().requires_grad_()
+        g = torch.randn(4, dim, generator=gen(3)).cuda()
+        alone, = torch.autograd.grad(embed_bags(table, tokens, offsets, w, mean=True, out_dtype=F32), w, g)
+        _, (_, both) = check_bags(table, tokens, offsets, w.detach(), mean=True, out_dtype=F32, grad=g)
+        assert torch.equal(alone, both)
+
+
+def test_weights_outside_every_bag_do_not_count():
+    table = torch.randn(9, 16, generator=gen(0)).cuda()
+    tokens = torch.randint(0, 9, (5000,), generator=gen(1)).cuda()
+    w = torch.rand(5000, generator=gen(2))
+    w[:7], w[4000:] = math.nan, math.inf
+    offsets = torch.tensor([7, 20, 20, 4000]).cuda()
+    inside = w.clone()
+    inside[:7] = inside[4000:] = 0.0
+    w, inside = w.cuda().requires_grad_(), inside.cuda().requires_grad_()
+    leaf, g = table.clone().requires_grad_(), torch.randn(3, 16, generator=gen(3)).cuda()
+    got, want = embed_bags(leaf, tokens, offsets, w, mean=True), embed_bags(leaf, tokens, offsets, inside, mean=True)
+    assert torch.equal(got, want) and torch.isfinite(got).all()
+    for a, b in zip(torch.autograd.grad(got, [leaf, w], g), torch.autograd.grad(want, [leaf, inside], g)):
+        assert torch.equal(a, b) and torch.isfinite(a).all()
+
+
+@pytest.mark.parametrize("n", [300, 9001])
+def test_offsets_outside_the_tokens(n):
+    """Ascending ones past both ends are the ends; of others the results are not specified, but
+    nothing else is touched."""
+    table = torch.randn(40, 24, generator=gen(0)).cuda().requires_grad_()
+    tokens = torch.randint(0, 40, (n,), generator=gen(1)).cuda()
+    offsets = torch.tensor([-2 ** 62, -5, 3, n // 2, n // 2, n + 9, 2 ** 62]).cuda()
+    g = torch.randn(6, 24, generator=gen(2)).cuda()
+    want = embed_bags(table, tokens, offsets.clamp(0, n), mean=True)
+    got = embed_bags(table, tokens, offsets, mean=True)
+    assert torch.equal(got, want)
+    d_want, = torch.autograd.grad(want, table, g)
+    assert torch.equal(torch.autograd.grad(got, table, g)[0], d_want)
+    for seed in range(3):
+        wild = torch.randint(-n, 2 * n, (7,), generator=gen(seed)).cuda()
+        wild[seed] = (-2 ** 63, 2 ** 63 - 1, 0)[seed]
+        torch.autograd.grad(embed_bags(table, tokens, wild, mean=True), table, g)
+    assert torch.equal(embed_bags(table, tokens, offsets, mean=True), want)
+
+
+def test_values_and_ids_of_32_bits():
+    x = some_logits(0, 9, 500, F32)
+    tokens = torch.randint(0, 500, (9,), generator=gen(1)).cuda()
+    ids, dist = found(2, 9, 20, 60)
+    values = torch.randint(-1, 501, (60,), generator=gen(3)).cuda()
+    want = token_logprobs(x, tokens, top=4, neighbours=Neighbours(ids, dist, values))
+    got = token_logprobs(x, tokens.int(), top=4, neighbours=Neighbours(ids.int(), dist, values.int()))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
