@@ -279,7 +279,7 @@ class IvfUsqIndex:
     def _check_vectors(self, t, what: str):
         if not getattr(t, "is_cuda", False) or t.device.index != self.device:
             raise ValueError(f"{what} must be a tensor on cuda:{self.device}")
-        if t.shape[-1] != self.config.dim:
+        if t.dim() == 0 or t.shape[-1] != self.config.dim:
             raise ValueError("query dimension mismatch")
 
     def search_tokens(self, table, tokens, offsets, req: SearchRequest, weights=None, *,
@@ -307,6 +307,8 @@ class IvfUsqIndex:
         from .tokens import Neighbours, token_logprobs
         import torch
         self._check_vectors(queries, "queries")
+        if not isinstance(tokens, torch.Tensor):
+            raise ValueError("tokens must be a tensor")
         if queries.dtype != torch.float32 or queries.shape[:-1] != tokens.shape:
             raise ValueError("queries must be float32, one vector per token")
         k = max(int(req.top_k), 1)

@@ -1122,3 +1122,14 @@ def test_values_and_ids_of_32_bits():
     want = token_logprobs(x, tokens, top=4, neighbours=Neighbours(ids, dist, values))
     got = token_logprobs(x, tokens.int(), top=4, neighbours=Neighbours(ids.int(), dist, values.int()))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_index_methods_refuse_what_is_no_matrix_or_no_tensor(small_index):
+    from hanns_b200 import SearchRequest
+    req, t = SearchRequest(top_k=3), torch.zeros(3, dtype=torch.long).cuda()
+    for bad in (lambda: small_index.search_tokens(torch.zeros(()).cuda(), t, torch.tensor([0, 3]).cuda(), req),
+                lambda: small_index.search_tokens(torch.zeros(64).cuda(), t, torch.tensor([0, 3]).cuda(), req),
+                lambda: small_index.token_logprobs(torch.zeros(()).cuda(), torch.zeros(9).cuda(), t[0], t, req),
+                lambda: small_index.token_logprobs(torch.zeros(3, 64).cuda(), torch.zeros(3, 9).cuda(), [0, 1, 2], t, req)):
+        with pytest.raises(ValueError):
+            bad()
