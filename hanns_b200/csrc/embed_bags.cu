@@ -47,8 +47,8 @@ constexpr int kLookupPacks = 8;       // vectors of a lane in a lookup
 constexpr int kMaxBinBits = 9, kMaxBins = 1 << kMaxBinBits;
 constexpr int kSortItems = 4, kSortTile = kThreads * kSortItems;
 // Up to so many tiles each adds up the counts of those before it itself, without a scan kernel between.
-// A gradient of 8 tiles takes 23.4 us for 26.2 then, 16 tiles 38.3 for 40.6, 32 tiles 35.8 either
-// way, 64 tiles 46.2 for 44.0.
+// The gradient of a lookup in 32,000 x 64 f32 (device time): 8 tiles of positions 29.8 us (with the scan
+// 32.4), 16 tiles 32.6 (34.5), 24 36.1 (37.4), 32 39.8 (39.9), 64 45.4 (43.0).
 constexpr int kFewTiles = 16;
 // Offsets to a position of a tile from which the positions search among them: 3,000 positions and
 // 70,000 bags sort in 20 us (marked 53), 16,000 bags 20 (23), 300 bags 16 (13.6 marked).
@@ -380,9 +380,9 @@ __device__ __forceinline__ void sum_segment(const SumArgs& a, const Lanes& ln, B
 }
 
 // Forward: one warp per (bag, column tile).  Bound by the gather through the L2 and the chain offsets
-// - tokens - rows: 150,001 tokens in 10,000 bags of a 768-wide bf16 table (230 MB of rows, 31 MB
-// of vectors) take 25 us, 9 TB/s.  Longest bag here 32: 25 + 15 us with the pieces, 64: 37 + 14,
-// 16: 21 + 30.
+// - tokens - rows: of 150,001 tokens in 10,000 bags of a 768-wide bf16 table this kernel's share
+// (198 MB through the L2, rows and vectors) takes 25 us, 8 TB/s.  Longest bag here 32: 25 + 15 us
+// with the pieces, 64: 37 + 14, 16: 21 + 30.
 template <class T, class TO, int VE, int Packs>
 __global__ void __launch_bounds__(kSegmentThreads, blocks_of_sm(Packs, VE, true))
     bags_kernel(SumArgs a, TokenEntries entries, BagSegments bags) {
@@ -1047,7 +1047,9 @@ struct Matrix {
 };
 
 // Elements per access that every row of the matrices allows: 16 bytes of the first one's, 8, 4, or
-// one element.
+// one element.  Forward, 150,001 tokens in 10,000 bags, with these accesses and with single elements:
+// 500 bf16 (4 at a time) 35 and 80 us, 502 bf16 (2) 46 and 80, 502 f32 (2) 52 and 87.  Both gradients of
+// f32 rows of 502 (2 at a time) take 188 and 183: there the single elements' wider tiles make up for it.
 int vector_elems(int dim, std::initializer_list<Matrix> all) {
     for (int ve = 16 / all.begin()->size; ve > 1; ve /= 2) {
         bool ok = dim % ve == 0;

@@ -808,7 +808,8 @@ __device__ __forceinline__ void dense_vector(const RowGrad& g, const Pack<float,
 }
 
 // Blocks take `span` vectors of a row each; its first block takes the partial ones at its ends.
-// Bound by memory: 4096 x 128,000 bf16 take 317 us, 6.6 TB/s.
+// Bound by memory: 4096 x 128,000 bf16 take 318 us, 6.6 TB/s (313 behind the forward call, whose last
+// logits are still in the L2).
 template <class T, bool Wide>
 __global__ void __launch_bounds__(kGradThreads, 12) logprobs_grad_kernel(GradArgs a) {
     wait_for_previous();
