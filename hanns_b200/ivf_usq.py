@@ -281,6 +281,11 @@ class IvfUsqIndex:
             raise ValueError(f"{what} must be a tensor on cuda:{self.device}")
         if t.dim() == 0 or t.shape[-1] != self.config.dim:
             raise ValueError("query dimension mismatch")
+        import torch
+        with torch.cuda.device(t.device):
+            # a replay would use the handle's buffers after a larger search has replaced them
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a search cannot be captured into a graph")
 
     def search_tokens(self, table, tokens, offsets, req: SearchRequest, weights=None, *,
                       scale: float = 1.0, mean: bool = True):

@@ -16,8 +16,9 @@
  * hanns_gpu_last_error() describes the last failure of the calling thread.
  * Calls on one handle are serialised by the handle: on the host by a mutex, on the device in
  * the order in which they were made, whatever streams they were given (the handle's buffers
- * are one call's after the other's).  A call that is captured into a graph is not: its
- * replays must not overlap other calls on the handle.
+ * are one call's after the other's).  A call that is captured into a graph takes no part: its
+ * replays must not overlap other calls on the handle, nor come after one for which the
+ * handle's buffers grew.
  */
 #ifndef HANNS_GPU_H
 #define HANNS_GPU_H

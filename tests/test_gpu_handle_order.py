@@ -164,3 +164,17 @@ def test_an_index_freed_behind_a_search_in_flight(own_stream):
     make_index(1000)  # takes what the index gave back
     torch.cuda.synchronize()
     assert same(got, want)
+
+
+def test_searches_are_not_captured(index):
+    import torch
+    args = batch(1, 100)
+    want = alone(index, args)
+    queries, logits, t = torch.randn(4, DIM).cuda(), torch.zeros(4, 9).cuda(), torch.zeros(4, dtype=torch.long).cuda()
+    for call in (lambda: index.search_tokens(*args, request()),
+                 lambda: index.token_logprobs(queries, logits, t, t, request())):
+        with pytest.raises(RuntimeError, match="captured"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    torch.cuda.synchronize()
+    assert same(index.search_tokens(*args, request()), want)
